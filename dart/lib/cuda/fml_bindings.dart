@@ -404,6 +404,18 @@ class FmlBindings {
   late final fmlOptimizerStep = lib.lookupFunction<
       Int32 Function(Pointer<FmlCtx>, Int32, Pointer<Float>, Pointer<Float>, Pointer<Float>, Pointer<Float>, Pointer<Float>, Int64, Double, Double, Double, Double, Double, Int32),
       int Function(Pointer<FmlCtx>, int, Pointer<Float>, Pointer<Float>, Pointer<Float>, Pointer<Float>, Pointer<Float>, int, double, double, double, double, double, int)>('fml_optimizer_step');
+  late final fmlAdamwStateFloats = lib.lookupFunction<
+      Int32 Function(Int32, Pointer<Int64>, Int32, Pointer<Int64>),
+      int Function(int, Pointer<Int64>, int, Pointer<Int64>)>('fml_adamw_state_floats');
+  late final fmlAdamwPlanCreate = lib.lookupFunction<
+      Int32 Function(Pointer<FmlCtx>, Int32, Pointer<Pointer<Float>>, Pointer<Pointer<Float>>, Pointer<Int64>, Pointer<Float>, Pointer<Float>, Int32, Pointer<Int32>),
+      int Function(Pointer<FmlCtx>, int, Pointer<Pointer<Float>>, Pointer<Pointer<Float>>, Pointer<Int64>, Pointer<Float>, Pointer<Float>, int, Pointer<Int32>)>('fml_adamw_plan_create');
+  late final fmlAdamwPlanStep = lib.lookupFunction<
+      Int32 Function(Pointer<FmlCtx>, Int32, Int32, Double, Double, Double, Double, Double, Int32, Double, Int32, Int64),
+      int Function(Pointer<FmlCtx>, int, int, double, double, double, double, double, int, double, int, int)>('fml_adamw_plan_step');
+  late final fmlAdamwPlanDestroy = lib.lookupFunction<
+      Int32 Function(Pointer<FmlCtx>, Int32),
+      int Function(Pointer<FmlCtx>, int)>('fml_adamw_plan_destroy');
   late final fmlAct2Fwd = lib.lookupFunction<
       Int32 Function(Pointer<FmlCtx>, Int32, Float, Pointer<Float>, Pointer<Float>, Int64),
       int Function(Pointer<FmlCtx>, int, double, Pointer<Float>, Pointer<Float>, int)>('fml_act2_fwd');

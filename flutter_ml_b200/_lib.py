@@ -131,6 +131,10 @@ PROTOTYPES = {
     "fml_adam_step": [fp, fp, fp, fp, fp, i64, C.c_double, C.c_double, C.c_double, C.c_double, i32, C.c_double],
     "fml_adam_step_on": [fp, i32, fp, fp, fp, fp, i64, C.c_double, C.c_double, C.c_double, C.c_double, i32, C.c_double, i32],
     "fml_optimizer_step": [fp, i32, fp, fp, fp, fp, fp, i64, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, i32],
+    "fml_adamw_state_floats": [i32, fp, i32, C.POINTER(i64)],
+    "fml_adamw_plan_create": [fp, i32, fp, fp, fp, fp, fp, i32, C.POINTER(i32)],
+    "fml_adamw_plan_step": [fp, i32, i32, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, i32, C.c_double, i32, i64],
+    "fml_adamw_plan_destroy": [fp, i32],
     "fml_act2_fwd": [fp, i32, f32, fp, fp, i64],
     "fml_act2_bwd": [fp, i32, f32, fp, fp, fp, i64, i32],
     "fml_attention_fwd": [fp, C.POINTER(AttentionDesc)],

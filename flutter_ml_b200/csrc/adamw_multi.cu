@@ -1,0 +1,382 @@
+// AdamW (lib/optimizers/adamw.dart:82-89) over a list of tensors in one launch, first and second moments in 32 or 8 bits.
+//
+// For every element, with g' = grad_scale g, c1 = 1 - beta1^t, c2 = 1 - beta2^t:
+//   m <- beta1 m + (1 - beta1) g'      v <- beta2 v + (1 - beta2) g'^2
+//   w <- w - lr (m / c1) / (sqrt(v / c2) + eps)        w <- w - lr weight_decay w
+//
+// Bound: memory, 28 bytes an element with 32-bit states (w, m, v read and written, g read), 16 with 8-bit ones.
+//
+// Layout: every tensor is cut into blocks of 256 elements, one warp a block, eight elements a lane (two float4: elements
+// 4 l .. 4 l + 3 and 128 + 4 l ..), all loads issued before the first use.  The states of all tensors lie in ONE buffer by
+// block, so they are aligned whatever the tensors' own addresses; parameters and gradients may start anywhere.  The list
+// becomes a table of work items on the device once, when the plan is made: a step is one launch whatever their number.
+//
+// 8-bit states.  m and r = sqrt(v) (v itself has twice the exponent range) are held as sign, four exponent and three
+// fraction bits times a power of two for each block, the smallest that brings the block's largest finite value to 448 at
+// most.  With a power of two every scaling is exact: the only rounding is that to three fraction bits, and a block's scale
+// changing does not move the values that it holds.  Values down to 2^-18 of the block's largest keep their precision or
+// part of it, smaller ones become zero; a positive r is held at 2^-9 of the scale at least, because m over a root that was
+// rounded to zero would be a step of any size.  beta2 = 0.999 changes v by a thousandth a step, far less than the half step
+// of 1/16 that rounding to the nearest takes away, so a v rounded that way stands still until a gradient beats it by an
+// order of magnitude: rounding up with the probability of the dropped bits (16 of them) keeps every state right on average.
+// The bits come from a counter (seed, step, block, element), so a run can be repeated exactly.  An element that is not
+// finite is held as NaN and left out of the block's scale: it damages nothing but itself.
+//
+// The moments are formed with one rounding an operation (no contraction), so a restatement in any IEEE float32 arithmetic
+// reproduces the codes bit for bit.
+#include <math.h>
+
+#include <algorithm>
+#include <new>
+#include <stdexcept>
+
+#include "common.cuh"
+
+namespace {
+
+constexpr int BLOCK = 256;                 // elements that share a scale, and a warp's work
+constexpr int WARPS = 8;
+constexpr int ITEM = BLOCK * WARPS;        // elements of a work item: one CTA
+
+struct Item {
+  float* w;
+  float* g;
+  uint32_t block;   // first block in the state buffers
+  uint32_t count;   // elements, 1 .. ITEM
+};
+
+struct Hyper {
+  float b1, omb1, b2, omb2;
+  float step;       // lr / (1 - beta1^t)
+  float rc2;        // 1 / sqrt(1 - beta2^t)
+  float eps, decay; // decay = lr * weight_decay
+  float gs;
+  uint32_t key;     // of the random bits
+};
+
+// Hyper-parameters before the step count enters; with them a device-side counter can be the step count.
+struct HyperIn {
+  double lr, beta1, beta2, eps, decay, gs;
+  int64_t seed;
+};
+
+__host__ __device__ inline uint32_t mix32(uint32_t x) {
+  x ^= x >> 16;
+  x *= 0x9E3779B1u;
+  x ^= x >> 15;
+  x *= 0x85EBCA77u;
+  return x ^ (x >> 13);
+}
+
+__host__ __device__ inline Hyper hyper_at(const HyperIn& p, int t) {
+  Hyper h;
+  h.b1 = (float)p.beta1; h.omb1 = (float)(1.0 - p.beta1);
+  h.b2 = (float)p.beta2; h.omb2 = (float)(1.0 - p.beta2);
+  h.step = (float)(p.lr / (1.0 - pow(p.beta1, (double)t)));
+  h.rc2 = (float)(1.0 / sqrt(1.0 - pow(p.beta2, (double)t)));
+  h.eps = (float)p.eps; h.decay = (float)(p.lr * p.decay); h.gs = (float)p.gs;
+  const uint64_t s = (uint64_t)p.seed;
+  h.key = mix32(mix32(mix32((uint32_t)s) ^ (uint32_t)(s >> 32)) ^ (uint32_t)t);
+  return h;
+}
+
+struct DeviceStep { Hyper h; int t; };   // the plan's own step counter, advanced on the device (captured launches included)
+__global__ void advance_kernel(DeviceStep* d, const HyperIn p) {
+  if (d->t < 0x7fffffff) d->t++;
+  d->h = hyper_at(p, d->t);
+}
+
+// value of a code in units of its scale: with the seven bits under the exponent's place and 2^120, subnormals come out right too
+__device__ __forceinline__ float decode8(uint32_t c) {
+  const float v = __uint_as_float((c & 0x7fu) << 20) * 0x1p120f;
+  return (c & 0x7fu) == 0x7fu ? __uint_as_float(0x7fc00000u) : __uint_as_float(__float_as_uint(v) | (c & 0x80u) << 24);
+}
+__device__ __forceinline__ bool finite_bits(uint32_t b) { return (b & 0x7fffffffu) < 0x7f800000u; }
+
+// exponent of the block's scale from the bits of its largest finite absolute value
+__device__ __forceinline__ int scale_exponent(uint32_t amax) { return max((int)((amax + 0x1FFFFFu) >> 23) - 135, -126); }
+
+// `y` = |x| / scale in [0, 448]; values below 2^-6 are moved up by 2^-6, where the steps of 2^-9 are float steps of the same
+// place, and back in the code
+template <bool NEAREST>
+__device__ __forceinline__ uint32_t encode8(float y, uint32_t rnd16) {
+  const bool small = y < 0x1p-6f;
+  const uint32_t z = __float_as_uint(small ? y + 0x1p-6f : y);
+  const uint32_t up = NEAREST ? 0x7FFFFu + ((z >> 20) & 1u) : rnd16 << 4;
+  return ((z + up) >> 20) - (small ? 968u : 960u);
+}
+
+template <bool EIGHT, bool NEAREST, bool ZERO>
+__global__ void __launch_bounds__(32 * WARPS) adamw_kernel(const Item* __restrict__ items, float* __restrict__ mbuf, float* __restrict__ vbuf,
+                                                           long long n_blocks, Hyper h, const DeviceStep* __restrict__ dev) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Item it = items[blockIdx.x];
+  const int n = (int)it.count - warp * BLOCK;   // elements left from this warp's block on
+  if (n <= 0) return;
+  const long long b = (long long)it.block + warp;
+  float* __restrict__ w = it.w + warp * BLOCK;
+  float* __restrict__ g = it.g + warp * BLOCK;
+  const bool vec = n >= BLOCK && ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(g)) & 15) == 0;
+  float wv[8], gv[8], mv[8], vv[8];
+  uint32_t mc[2], rc[2];
+  float ms = 0.f, rs = 0.f;
+  if (vec) {
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+      reinterpret_cast<float4*>(wv)[q] = reinterpret_cast<const float4*>(w)[lane + 32 * q];
+      reinterpret_cast<float4*>(gv)[q] = reinterpret_cast<const float4*>(g)[lane + 32 * q];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int i = (j >> 2) * 128 + 4 * lane + (j & 3);
+      wv[j] = i < n ? w[i] : 0.f;
+      gv[j] = i < n ? g[i] : 0.f;
+    }
+  }
+  if (EIGHT) {
+    const uint32_t* mw = reinterpret_cast<const uint32_t*>(mbuf) + b * (BLOCK / 4);
+    const uint32_t* rw = reinterpret_cast<const uint32_t*>(vbuf) + b * (BLOCK / 4);
+#pragma unroll
+    for (int q = 0; q < 2; q++) { mc[q] = mw[lane + 32 * q]; rc[q] = rw[lane + 32 * q]; }
+    ms = mbuf[n_blocks * (BLOCK / 4) + b];
+    rs = vbuf[n_blocks * (BLOCK / 4) + b];
+  } else {
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+      reinterpret_cast<float4*>(mv)[q] = reinterpret_cast<const float4*>(mbuf + b * BLOCK)[lane + 32 * q];
+      reinterpret_cast<float4*>(vv)[q] = reinterpret_cast<const float4*>(vbuf + b * BLOCK)[lane + 32 * q];
+    }
+  }
+  if (dev) h = dev->h;
+  float root[8];
+  uint32_t mmax = 0, rmax = 0;
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    float m, v;
+    if (EIGHT) {
+      m = __fmul_rn(decode8(mc[j >> 2] >> (8 * (j & 3)) & 0xffu), ms);
+      const float r = __fmul_rn(decode8(rc[j >> 2] >> (8 * (j & 3)) & 0xffu), rs);
+      v = __fmul_rn(r, r);
+    } else {
+      m = mv[j];
+      v = vv[j];
+    }
+    const float gj = __fmul_rn(gv[j], h.gs);
+    m = __fadd_rn(__fmul_rn(m, h.b1), __fmul_rn(gj, h.omb1));
+    v = __fadd_rn(__fmul_rn(v, h.b2), __fmul_rn(__fmul_rn(gj, gj), h.omb2));
+    root[j] = __fsqrt_rn(v);
+    // the quotient to two units in the last place: it moves w by lr times that
+    wv[j] -= __fdividef(h.step * m, fmaf(root[j], h.rc2, h.eps));
+    wv[j] -= h.decay * wv[j];
+    mv[j] = m;
+    vv[j] = v;
+    if (EIGHT) {
+      const uint32_t mb = __float_as_uint(m) & 0x7fffffffu, rb = __float_as_uint(root[j]);
+      mmax = max(mmax, finite_bits(mb) ? mb : 0u);
+      rmax = max(rmax, finite_bits(rb) ? rb : 0u);
+    }
+  }
+  if (vec) {
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+      reinterpret_cast<float4*>(w)[lane + 32 * q] = reinterpret_cast<float4*>(wv)[q];
+      if (ZERO) reinterpret_cast<float4*>(g)[lane + 32 * q] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int i = (j >> 2) * 128 + 4 * lane + (j & 3);
+      if (i < n) {
+        w[i] = wv[j];
+        if (ZERO) g[i] = 0.f;
+      }
+    }
+  }
+  if (!EIGHT) {   // places behind a tensor's last element in its last block: m = v = 0 stays so
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+      reinterpret_cast<float4*>(mbuf + b * BLOCK)[lane + 32 * q] = reinterpret_cast<float4*>(mv)[q];
+      reinterpret_cast<float4*>(vbuf + b * BLOCK)[lane + 32 * q] = reinterpret_cast<float4*>(vv)[q];
+    }
+    return;
+  }
+  const int me = scale_exponent(__reduce_max_sync(0xffffffffu, mmax)), re = scale_exponent(__reduce_max_sync(0xffffffffu, rmax));
+  const float mi = __int_as_float((127 - me) << 23), ri = __int_as_float((127 - re) << 23);
+  const uint32_t key = NEAREST ? 0u : mix32(h.key + (uint32_t)b * 0x9E3779B1u);
+  uint32_t mo[2] = {0, 0}, ro[2] = {0, 0};
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const uint32_t word = NEAREST ? 0u : mix32(key + (j >> 2) * 128 + 4 * lane + (j & 3));
+    const uint32_t mb = __float_as_uint(mv[j]), rb = __float_as_uint(root[j]);
+    uint32_t cm = encode8<NEAREST>(__fmul_rn(fabsf(mv[j]), mi), word >> 16);
+    uint32_t cr = encode8<NEAREST>(__fmul_rn(root[j], ri), word & 0xffffu);
+    cm = (finite_bits(mb) ? cm : 0x7fu) | (mb >> 31) << 7;
+    if (cr == 0 && root[j] > 0.f) cr = 1;
+    cr = finite_bits(rb) ? cr : 0x7fu;
+    mo[j >> 2] |= cm << (8 * (j & 3));
+    ro[j >> 2] |= cr << (8 * (j & 3));
+  }
+  uint32_t* mw = reinterpret_cast<uint32_t*>(mbuf) + b * (BLOCK / 4);
+  uint32_t* rw = reinterpret_cast<uint32_t*>(vbuf) + b * (BLOCK / 4);
+#pragma unroll
+  for (int q = 0; q < 2; q++) { mw[lane + 32 * q] = mo[q]; rw[lane + 32 * q] = ro[q]; }
+  if (lane == 0) {
+    mbuf[n_blocks * (BLOCK / 4) + b] = __int_as_float((me + 127) << 23);
+    vbuf[n_blocks * (BLOCK / 4) + b] = __int_as_float((re + 127) << 23);
+  }
+}
+
+int64_t blocks_of(int64_t n) { return (n + BLOCK - 1) / BLOCK; }
+
+// Total number of blocks, or -1 (bad arguments) / -2 (more than the 32-bit block counter holds)
+int64_t total_blocks(int32_t n, const int64_t* sizes) {
+  if (n < 1 || !sizes) return -1;
+  int64_t total = 0;
+  for (int32_t i = 0; i < n; i++) {
+    if (sizes[i] < 0) return -1;
+    if (sizes[i] > ((int64_t)1 << 39)) return -2;
+    total += blocks_of(sizes[i]);
+    if (total > 0x7fffffff) return -2;
+  }
+  return total;
+}
+
+}  // namespace
+
+struct fml_adamw_plan {
+  Item* items = nullptr;
+  DeviceStep* step = nullptr;
+  float *m = nullptr, *v = nullptr;
+  int64_t n_blocks = 0;
+  uint32_t n_items = 0;
+  int bits = 32;
+};
+
+static void free_plan(fml_adamw_plan* p) {
+  if (p->items) cudaFree(p->items);
+  if (p->step) cudaFree(p->step);
+  delete p;
+}
+void fml_adamw_release(fml_ctx* ctx) {
+  for (fml_adamw_plan* p : ctx->adamw_plans)
+    if (p) free_plan(p);
+  ctx->adamw_plans.clear();
+}
+
+extern "C" {
+
+int32_t fml_adamw_state_floats(int32_t n, const int64_t* sizes, int32_t state_bits, int64_t* floats) {
+  if (!floats || (state_bits != 8 && state_bits != 32)) return fml_fail(nullptr, FML_ERR_INVALID, "fml_adamw_state_floats: bad arguments");
+  const int64_t nb = total_blocks(n, sizes);
+  if (nb < 0) return fml_fail(nullptr, nb == -1 ? FML_ERR_INVALID : FML_ERR_OOM, "fml_adamw_state_floats: bad tensor sizes");
+  *floats = state_bits == 32 ? nb * BLOCK : nb * (BLOCK / 4 + 1);
+  return FML_OK;
+}
+
+int32_t fml_adamw_plan_create(fml_ctx* ctx, int32_t n, float* const* w, float* const* g, const int64_t* sizes, float* m, float* v,
+                              int32_t state_bits, int32_t* plan_id) {
+  if (plan_id) *plan_id = -1;
+  FML_REQUIRE(ctx, ctx && w && g && plan_id, "fml_adamw_plan_create: bad arguments");
+  FML_REQUIRE(ctx, state_bits == 8 || state_bits == 32, "fml_adamw_plan_create: states are held in 8 or 32 bits");
+  FML_REQUIRE(ctx, !ctx->capturing, "fml_adamw_plan_create: make the plan before the recording starts");
+  FML_ENTER(ctx);
+  const int64_t nb = total_blocks(n, sizes);
+  FML_REQUIRE(ctx, nb != -1, "fml_adamw_plan_create: bad tensor sizes");
+  if (nb == -2) return fml_fail(ctx, FML_ERR_OOM, "fml_adamw_plan_create: too many elements for one plan");
+  FML_REQUIRE(ctx, nb == 0 || (m && v), "fml_adamw_plan_create: missing state buffer");
+  FML_REQUIRE(ctx, ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 15) == 0,
+              "fml_adamw_plan_create: state buffers must be 16-byte aligned");
+  fml_adamw_plan* p = nullptr;
+  try {
+    struct Range { uintptr_t a, e; };
+    std::vector<Range> used;
+    std::vector<Item> items;
+    const uintptr_t sb = (uintptr_t)(state_bits == 32 ? nb * BLOCK : nb * (BLOCK / 4 + 1)) * 4;
+    if (nb) {
+      used.push_back({reinterpret_cast<uintptr_t>(m), reinterpret_cast<uintptr_t>(m) + sb});
+      used.push_back({reinterpret_cast<uintptr_t>(v), reinterpret_cast<uintptr_t>(v) + sb});
+    }
+    uint32_t block = 0;
+    for (int32_t i = 0; i < n; i++) {
+      if (sizes[i] == 0) continue;
+      FML_REQUIRE(ctx, w[i] && g[i], "fml_adamw_plan_create: missing tensor or gradient");
+      FML_REQUIRE(ctx, ((reinterpret_cast<uintptr_t>(w[i]) | reinterpret_cast<uintptr_t>(g[i])) & 3) == 0,
+                  "fml_adamw_plan_create: misaligned tensor or gradient");
+      for (const float* q : {w[i], g[i]}) used.push_back({reinterpret_cast<uintptr_t>(q), reinterpret_cast<uintptr_t>(q + sizes[i])});
+      for (int64_t o = 0; o < sizes[i]; o += ITEM, block += WARPS)
+        items.push_back({w[i] + o, g[i] + o, block, (uint32_t)std::min<int64_t>(ITEM, sizes[i] - o)});
+      block -= (uint32_t)((WARPS - blocks_of(sizes[i]) % WARPS) % WARPS);   // the last item's missing blocks
+    }
+    for (const Range& r : used) {
+      cudaPointerAttributes a;
+      FML_CUDA(ctx, cudaPointerGetAttributes(&a, reinterpret_cast<const void*>(r.a)));
+      FML_REQUIRE(ctx, (a.type == cudaMemoryTypeDevice && a.device == ctx->device) || a.type == cudaMemoryTypeManaged,
+                  "fml_adamw_plan_create: a buffer is not in the memory of the context's device");
+    }
+    std::sort(used.begin(), used.end(), [](const Range& x, const Range& y) { return x.a < y.a; });
+    for (size_t i = 1; i < used.size(); i++)
+      FML_REQUIRE(ctx, used[i - 1].e <= used[i].a, "fml_adamw_plan_create: tensors, gradients and states must not overlap");
+    p = new fml_adamw_plan();
+    p->m = m; p->v = v; p->n_blocks = nb; p->n_items = (uint32_t)items.size(); p->bits = state_bits;
+    cudaError_t e = cudaMalloc(&p->step, sizeof(DeviceStep));
+    if (e == cudaSuccess) e = cudaMemset(p->step, 0, sizeof(DeviceStep));
+    if (e == cudaSuccess && !items.empty()) e = cudaMalloc(&p->items, items.size() * sizeof(Item));
+    if (e == cudaSuccess && !items.empty()) e = cudaMemcpy(p->items, items.data(), items.size() * sizeof(Item), cudaMemcpyHostToDevice);
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();   // the table is there whatever stream the first step runs on
+    if (e != cudaSuccess) {
+      free_plan(p);
+      return fml_fail(ctx, e == cudaErrorMemoryAllocation ? FML_ERR_OOM : FML_ERR_CUDA, std::string("fml_adamw_plan_create: ") + cudaGetErrorString(e));
+    }
+    ctx->adamw_plans.push_back(p);
+  } catch (const std::exception&) {
+    if (p) free_plan(p);
+    return fml_fail(ctx, FML_ERR_OOM, "fml_adamw_plan_create: out of host memory");
+  }
+  *plan_id = (int32_t)ctx->adamw_plans.size() - 1;
+  return FML_OK;
+}
+
+int32_t fml_adamw_plan_step(fml_ctx* ctx, int32_t plan_id, int32_t lane, double lr, double beta1, double beta2, double eps,
+                            double weight_decay, int32_t t, double grad_scale, int32_t zero_grad, int64_t seed) {
+  FML_REQUIRE(ctx, ctx, "fml_adamw_plan_step: no context");
+  FML_ENTER(ctx);
+  FML_REQUIRE(ctx, plan_id >= 0 && plan_id < (int32_t)ctx->adamw_plans.size() && ctx->adamw_plans[plan_id], "fml_adamw_plan_step: unknown plan");
+  FML_REQUIRE(ctx, beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, "fml_adamw_plan_step: betas must be in [0, 1)");
+  FML_REQUIRE(ctx, eps > 0 && isfinite(eps) && isfinite(lr) && isfinite(weight_decay) && isfinite(grad_scale),
+              "fml_adamw_plan_step: hyper-parameters must be finite, eps positive");
+  FML_REQUIRE(ctx, t >= 0, "fml_adamw_plan_step: t must be >= 1, or 0 for the plan's own counter");
+  cudaStream_t s;
+  const int32_t rc = fml_any_stream(ctx, lane, &s);
+  if (rc) return rc;
+  const fml_adamw_plan* p = ctx->adamw_plans[plan_id];
+  const HyperIn in = {lr, beta1, beta2, eps, weight_decay, grad_scale, seed};
+  const DeviceStep* dev = nullptr;
+  if (t == 0) {
+    advance_kernel<<<1, 1, 0, s>>>(p->step, in);
+    FML_LAUNCH_CHECK(ctx, "advance_kernel");
+    dev = p->step;
+  }
+  if (p->n_items == 0) return FML_OK;
+  const Hyper h = hyper_at(in, t ? t : 1);
+  const bool nearest = seed < 0, zero = zero_grad != 0;
+  auto* k = p->bits == 32 ? (zero ? adamw_kernel<false, true, true> : adamw_kernel<false, true, false>)
+            : nearest     ? (zero ? adamw_kernel<true, true, true> : adamw_kernel<true, true, false>)
+                          : (zero ? adamw_kernel<true, false, true> : adamw_kernel<true, false, false>);
+  k<<<p->n_items, 32 * WARPS, 0, s>>>(p->items, p->m, p->v, p->n_blocks, h, dev);
+  FML_LAUNCH_CHECK(ctx, "adamw_kernel");
+  return FML_OK;
+}
+
+int32_t fml_adamw_plan_destroy(fml_ctx* ctx, int32_t plan_id) {
+  FML_REQUIRE(ctx, ctx, "fml_adamw_plan_destroy: no context");
+  FML_ENTER(ctx);
+  FML_REQUIRE(ctx, plan_id >= 0 && plan_id < (int32_t)ctx->adamw_plans.size() && ctx->adamw_plans[plan_id], "fml_adamw_plan_destroy: unknown plan");
+  FML_REQUIRE(ctx, !ctx->capturing, "fml_adamw_plan_destroy: not while a graph is being recorded");
+  FML_CUDA(ctx, cudaDeviceSynchronize());   // steps may still run on the main stream or on any lane
+  free_plan(ctx->adamw_plans[plan_id]);
+  ctx->adamw_plans[plan_id] = nullptr;
+  return FML_OK;
+}
+
+}  // extern "C"

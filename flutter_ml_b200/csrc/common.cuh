@@ -15,6 +15,8 @@
 
 #include "fml.h"
 
+struct fml_adamw_plan;  // adamw_multi.cu
+
 struct fml_ctx {
   int device = 0;
   int sm_count = 0;
@@ -32,6 +34,7 @@ struct fml_ctx {
   cudaStream_t lanes[4] = {nullptr, nullptr, nullptr, nullptr};  // side streams (copies, exchange), created on first use
   std::vector<cudaGraphExec_t> graphs;         // instantiated graphs, index = graph id
   bool capturing = false;
+  std::vector<fml_adamw_plan*> adamw_plans;    // index = plan id; NULL once destroyed
   int sm_reserve = 0;  // SMs the persistent tensor-core kernels leave free (fml_set_sm_reserve)
   int last_gemm_path = 0;
   int last_gemm_tile[4] = {0, 0, 0, 0};  // of the last tensor-core launch: CTAs per tile (1 or 2), tile columns, K splits, K chunks
@@ -120,6 +123,7 @@ struct fml_lstm_epilogue {
 };
 
 // internal entry points between translation units
+void fml_adamw_release(fml_ctx* ctx);  // frees every optimizer plan of a context that is being shut down
 int32_t fml_gemm_tc(fml_ctx* ctx, const fml_gemm_desc* d, int precision, const fml_lstm_epilogue* lstm = nullptr);
 int32_t fml_gemm_simt(fml_ctx* ctx, const fml_gemm_desc* d);
 bool fml_gemm_tc_eligible(const fml_gemm_desc* d);

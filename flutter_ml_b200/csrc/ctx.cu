@@ -140,6 +140,7 @@ int32_t fml_shutdown(fml_ctx* ctx) {
   fml_dp_shutdown(ctx);
   for (void* p : ctx->allocs) cudaFreeAsync(p, ctx->stream);
   cudaStreamSynchronize(ctx->stream);
+  fml_adamw_release(ctx);
   if (ctx->ws) cudaFree(ctx->ws);
   cudaFree(ctx->d_status);
   cudaEventDestroy(ctx->ev0);

@@ -6,6 +6,8 @@ DenseLayerMatrix convention: activations are [rows x features], weights [in x ou
 """
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 
 from . import _lib
@@ -171,3 +173,51 @@ class DenseFwdBwdHost:
         for k, src in (("C", self.C), ("dA", self.dA), ("dB", self.dB), ("dbias", self.dbias)):
             c.download_into(src, self.h_out[k])  # the last one synchronises
         return self.h_out
+
+
+class AdamWPlan:
+    """AdamW (lib/optimizers/adamw.dart:82-89) over a list of tensors in one launch (`fml_adamw_plan_*`).  `w` and `g` are
+    lists of device arrays, `m` and `v` the two state buffers of `state_floats(sizes, stateBits)` floats, zeroed before the
+    first step; all must keep their addresses while the plan lives (the plan holds a reference to each)."""
+
+    def __init__(self, ctx, w, g, m, v, stateBits: int = 32):
+        if len(w) != len(g) or any(a.size != b.size for a, b in zip(w, g)):
+            raise ValueError("AdamWPlan: every tensor needs a gradient of its size")
+        if any(a.dtype != np.float32 for a in (*w, *g, m, v)):
+            raise ValueError("AdamWPlan: tensors, gradients and states are float32 buffers")
+        sizes = [a.size for a in w]
+        need = self.state_floats(sizes, stateBits)
+        if m.size < need or v.size < need:
+            raise ValueError(f"AdamWPlan: the state buffers need {need} floats")
+        self.ctx, self._keep, self.id, self.stateBits = ctx, (list(w), list(g), m, v), -1, stateBits
+        n = len(w)
+        wp, gp = np.array([a.ptr for a in w], dtype=np.uint64), np.array([a.ptr for a in g], dtype=np.uint64)
+        sz, pid = np.array(sizes, dtype=np.int64), ctypes.c_int32(-1)
+        ctx.check(ctx.lib.fml_adamw_plan_create(ctx.h, n, wp.ctypes.data, gp.ctypes.data, sz.ctypes.data, m.ptr, v.ptr, stateBits,
+                                                ctypes.byref(pid)))
+        self.id = pid.value
+
+    @staticmethod
+    def state_floats(sizes, stateBits: int = 32) -> int:
+        """Floats of each of the two state buffers for tensors of these element counts."""
+        lib, sz, out = _lib.load(), np.array(sizes, dtype=np.int64), ctypes.c_int64(0)
+        if lib.fml_adamw_state_floats(len(sz), sz.ctypes.data, stateBits, ctypes.byref(out)) != 0:
+            raise _lib.FmlError(lib.fml_last_error(None).decode())
+        return out.value
+
+    def step(self, lr, beta1, beta2, epsilon, weightDecay, t, grad_scale=1.0, zero_grad=False, seed=-1, lane=-1):
+        """One update; t = 0 counts on the device (for recorded steps), seed >= 0 rounds 8-bit states at random."""
+        self.ctx.check(self.ctx.lib.fml_adamw_plan_step(self.ctx.h, self.id, lane, lr, beta1, beta2, epsilon, weightDecay, t, grad_scale,
+                                                        1 if zero_grad else 0, seed))
+        self.ctx.launches += 1 if t else 2
+
+    def close(self):
+        if self.id >= 0 and self.ctx.h:
+            self.ctx.check(self.ctx.lib.fml_adamw_plan_destroy(self.ctx.h, self.id))
+        self.id = -1
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass

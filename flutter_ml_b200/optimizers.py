@@ -11,6 +11,7 @@ from typing import List, Optional
 
 import numpy as np
 
+from .ops import AdamWPlan
 from .tensor import Tensor
 
 
@@ -209,3 +210,53 @@ class AMSGrad(_StatefulOptimizer):
 
     def _hyper(self):
         return (self.beta1, self.beta2, self.epsilon)
+
+
+class MultiTensorAdamW(Optimizer):
+    """`AdamW` for parameters that are not packed into an arena: one launch for the whole list instead of one a tensor, the
+    moments in 32 bits or in 8 (a quarter of the state memory; `fml_adamw_plan_create` describes the format).
+
+    stateBits=8 rounds the moments at random by `seed` (the same seed repeats a run exactly) unless `seed` is None, which
+    rounds to the nearest code.  Gradients that do not exist yet are created, zeroed, here.  `step()` looks at the tensors'
+    and gradients' addresses and makes its plan anew where one has changed.  deviceCounter=True keeps the step count on the
+    device, so that a recorded step (`graph_begin`) advances it at every replay."""
+
+    def __init__(self, parameters, learningRate, beta1=0.9, beta2=0.999, epsilon=1e-8, weightDecay=0.01, stateBits=32,
+                 seed: Optional[int] = 0, deviceCounter: bool = False):
+        super().__init__(list(parameters), learningRate, None)
+        if not self.parameters:
+            raise ValueError("MultiTensorAdamW: no parameters")
+        if seed is not None and seed < 0:
+            raise ValueError("MultiTensorAdamW: seed must not be negative (None rounds to the nearest)")
+        self.beta1, self.beta2, self.epsilon, self.weightDecay = beta1, beta2, epsilon, weightDecay
+        self.stateBits, self.seed, self.deviceCounter, self._t = stateBits, seed, deviceCounter, 0
+        self.ctx = self.parameters[0].ctx
+        self._sizes = [p.value.size for p in self.parameters]
+        n = AdamWPlan.state_floats(self._sizes, stateBits)
+        self._m, self._v = self.ctx.zeros(n), self.ctx.zeros(n)
+        for p in self.parameters:
+            if p.grad is None:
+                p.zeroGrad()
+        self._plan, self._at = None, None
+        self._current_plan()
+
+    def _current_plan(self):
+        if any(p.grad is None for p in self.parameters):
+            raise ValueError("MultiTensorAdamW: a parameter has no gradient")
+        at = [(p.value.ptr, p.grad.ptr) for p in self.parameters]
+        if at != self._at:
+            if self.deviceCounter and self._plan is not None:
+                raise ValueError("MultiTensorAdamW: parameters and gradients must stay where they are while the device counts the steps")
+            if [p.value.size for p in self.parameters] != self._sizes:
+                raise ValueError("MultiTensorAdamW: a parameter has changed its size")
+            plan = AdamWPlan(self.ctx, [p.value for p in self.parameters], [p.grad for p in self.parameters], self._m, self._v, self.stateBits)
+            if self._plan is not None:
+                self._plan.close()
+            self._plan, self._at = plan, at
+        return self._plan
+
+    def step(self, grad_scale: float = 1.0, zero_grad: bool = False):
+        plan = self._current_plan()
+        self._t += 1
+        plan.step(self.learningRate, self.beta1, self.beta2, self.epsilon, self.weightDecay, 0 if self.deviceCounter else self._t,
+                  grad_scale, zero_grad, -1 if self.seed is None else self.seed)

@@ -339,6 +339,29 @@ typedef enum { FML_OPT_MOMENTUM = 1, FML_OPT_NAG = 2, FML_OPT_RMSPROP = 3, FML_O
 int32_t fml_optimizer_step(fml_ctx* ctx, int32_t kind, float* w, const float* g, float* s1, float* s2, float* s3,
                            int64_t n, double lr, double h1, double h2, double h3, double h4, int32_t t);
 
+/* AdamW (FML_OPT_ADAMW's rule) over a whole list of tensors in one launch, the moments in 32 or in 8 bits.
+ * A plan holds what stays the same from step to step: the tensors, their gradients and the two state buffers.
+ *   w, g, sizes  host arrays of n entries: device pointers (any 4-byte aligned address) and element counts; an entry of
+ *                size 0 is skipped.  No two of all these buffers may overlap, and all must be in the device's memory.
+ *   m, v         one buffer each for the whole list, 16-byte aligned, of fml_adamw_state_floats floats, zeroed before the
+ *                first step.  Tensor i owns the blocks of 256 elements that follow those of tensor i - 1 (its last block may
+ *                be partly unused).  32 bits: m and v, 256 floats a block.  8 bits: first the codes of all blocks, 256
+ *                bytes each (sign, 4 exponent and 3 fraction bits, 0x7f NaN), then one float32 scale, a power of two, for
+ *                each block; an element is code * scale, and the second buffer holds sqrt(v).
+ * A plan belongs to its context, which frees those that are left at fml_shutdown; it must outlive the graphs that were
+ * recorded with it.  Make and destroy plans outside recordings (both wait for the device). */
+int32_t fml_adamw_state_floats(int32_t n, const int64_t* sizes, int32_t state_bits, int64_t* floats);
+int32_t fml_adamw_plan_create(fml_ctx* ctx, int32_t n, float* const* w, float* const* g, const int64_t* sizes, float* m,
+                              float* v, int32_t state_bits, int32_t* plan_id);
+/* One step on copy lane `lane` (-1: the main stream).  t >= 1 is the step count after the increment, as in fml_adam_step;
+ * t = 0 counts the plan's steps on the device, so that every replay of a recorded step advances the count.  grad_scale
+ * multiplies g first; zero_grad != 0 clears g in the same pass.  seed concerns 8-bit states only: negative rounds to the
+ * nearest code, any other value rounds up or down at random with the probabilities that keep the mean, from a generator
+ * over (seed, t, block, element) - the same call gives the same bits.  eps must be positive, betas in [0, 1). */
+int32_t fml_adamw_plan_step(fml_ctx* ctx, int32_t plan_id, int32_t lane, double lr, double beta1, double beta2, double eps,
+                            double weight_decay, int32_t t, double grad_scale, int32_t zero_grad, int64_t seed);
+int32_t fml_adamw_plan_destroy(fml_ctx* ctx, int32_t plan_id);
+
 /* The other activations of lib/activationFunctions, with their parameter: FML_ACT2_LEAKY_RELU (alpha, leakyRelu.dart:35-48),
  * FML_ACT2_ELU (alpha, elu.dart:27-41), FML_ACT2_SWISH (silu.dart:29-49), FML_ACT2_MISH (mish.dart:29-31).
  * Backward takes the INPUT x and adds into dx when accumulate != 0. */
