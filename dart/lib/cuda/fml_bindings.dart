@@ -93,6 +93,7 @@ abstract final class FmlTapeDirection {
 
 abstract final class FmlLimits {
   static const int FML_XENT_STATIC_MAX_ROWS = 65536;
+  static const int FML_QK_NORM_ROPE_PARTS = 592;
 }
 
 /// `fml_config` of include/fml.h (16 bytes).
@@ -434,6 +435,12 @@ class FmlBindings {
   late final fmlAttentionBwd = lib.lookupFunction<
       Int32 Function(Pointer<FmlCtx>, Pointer<FmlAttentionDesc>, Pointer<Float>, Int64, Pointer<Float>, Pointer<Float>, Pointer<Float>, Int64, Int32, Pointer<Float>),
       int Function(Pointer<FmlCtx>, Pointer<FmlAttentionDesc>, Pointer<Float>, int, Pointer<Float>, Pointer<Float>, Pointer<Float>, int, int, Pointer<Float>)>('fml_attention_bwd');
+  late final fmlQkNormRopeFwd = lib.lookupFunction<
+      Int32 Function(Pointer<FmlCtx>, Pointer<Float>, Int64, Pointer<Float>, Int64, Int32, Pointer<Float>, Int64, Pointer<Float>, Int64, Int32, Int64, Int32, Pointer<Float>, Pointer<Float>, Pointer<Int32>, Int32, Int32, Int32, Double, Float),
+      int Function(Pointer<FmlCtx>, Pointer<Float>, int, Pointer<Float>, int, int, Pointer<Float>, int, Pointer<Float>, int, int, int, int, Pointer<Float>, Pointer<Float>, Pointer<Int32>, int, int, int, double, double)>('fml_qk_norm_rope_fwd');
+  late final fmlQkNormRopeBwd = lib.lookupFunction<
+      Int32 Function(Pointer<FmlCtx>, Pointer<Float>, Int64, Pointer<Float>, Int64, Pointer<Float>, Int64, Int32, Pointer<Float>, Int64, Pointer<Float>, Int64, Pointer<Float>, Int64, Int32, Int64, Int32, Pointer<Float>, Pointer<Float>, Pointer<Float>, Pointer<Float>, Pointer<Int32>, Int32, Int32, Int32, Double, Float, Int32, Pointer<Float>),
+      int Function(Pointer<FmlCtx>, Pointer<Float>, int, Pointer<Float>, int, Pointer<Float>, int, int, Pointer<Float>, int, Pointer<Float>, int, Pointer<Float>, int, int, int, int, Pointer<Float>, Pointer<Float>, Pointer<Float>, Pointer<Float>, Pointer<Int32>, int, int, int, double, double, int, Pointer<Float>)>('fml_qk_norm_rope_bwd');
   late final fmlConv2dFwd = lib.lookupFunction<
       Int32 Function(Pointer<FmlCtx>, Pointer<Float>, Pointer<Float>, Pointer<Float>, Pointer<Float>, Int32, Int32, Int32, Int32, Int32, Int32, Int32),
       int Function(Pointer<FmlCtx>, Pointer<Float>, Pointer<Float>, Pointer<Float>, Pointer<Float>, int, int, int, int, int, int, int)>('fml_conv2d_fwd');

@@ -20,6 +20,8 @@ ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_TANH, ACT_GELU = 0, 1, 2, 3, 4
 ACT_BY_NAME = {None: ACT_NONE, "none": ACT_NONE, "relu": ACT_RELU, "sigmoid": ACT_SIGMOID, "tanh": ACT_TANH,
                "gelu": ACT_GELU}
 
+QK_NORM_ROPE_PARTS = 592   # partial sums of the gain gradients, one a CTA (FML_QK_NORM_ROPE_PARTS)
+
 i32, i64, f32 = C.c_int32, C.c_int64, C.c_float
 fp = C.c_void_p  # device pointers travel as plain addresses
 
@@ -139,6 +141,9 @@ PROTOTYPES = {
     "fml_act2_bwd": [fp, i32, f32, fp, fp, fp, i64, i32],
     "fml_attention_fwd": [fp, C.POINTER(AttentionDesc)],
     "fml_attention_bwd": [fp, C.POINTER(AttentionDesc), fp, i64, fp, fp, fp, i64, i32, fp],
+    "fml_qk_norm_rope_fwd": [fp, fp, i64, fp, i64, i32, fp, i64, fp, i64, i32, i64, i32, fp, fp, fp, i32, i32, i32, C.c_double, f32],
+    "fml_qk_norm_rope_bwd": [fp, fp, i64, fp, i64, fp, i64, i32, fp, i64, fp, i64, fp, i64, i32, i64, i32, fp, fp, fp, fp, fp, i32, i32, i32,
+                             C.c_double, f32, i32, fp],
     "fml_conv2d_fwd": [fp, fp, fp, fp, fp, i32, i32, i32, i32, i32, i32, i32],
     "fml_conv2d_bwd": [fp, fp, fp, fp, fp, fp, fp, i32, i32, i32, i32, i32, i32, i32],
     "fml_checkpoint_save": [fp, C.c_char_p, i64, i32, fp, fp, fp],

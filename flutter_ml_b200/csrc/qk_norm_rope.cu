@@ -1,0 +1,497 @@
+// Root-mean-square norm of every query and key head, its gain, and the position rotation, in one pass; and the backward
+// pass.  It stands between the projections and the attention kernels (lib/layertypes/singleHeadAttentionLayer.dart:77-86
+// has neither; an extension).
+//
+//   r = 1 / sqrt(mean(x^2) + eps)    xh = x r    z = gain xh    y = R(pos) z
+//   R turns the pairs of the first rot_dim elements by pos base^(-2 i / rot_dim): pairs (i, i + rot_dim / 2), or neighbours
+//   dz = R^T dy    dgain += sum dz xh    dx = r (gain dz - xh mean(gain dz xh))
+//
+// Bound: memory, 8 bytes an element forward (x in, y out), 12 backward (x, dy in, dx out).  Nothing is saved between the
+// two passes: r comes again from the head, which the backward pass has in registers anyway.
+//
+// Layout: 4, 8, 16 or 32 lanes hold a head (d_head up to 32, 64, 128, 256), eight elements each: two float4, in the rotated
+// part four elements of its first half and their partners of the second, so a pair never leaves its lane; the only exchange
+// is the reduction.  A warp takes 32 / lanes heads of a row at once, queries and keys alike, and its next items' loads go
+// out before the first is used.  The cosines and sines of a CTA's rows are formed once, into shared memory, for all heads:
+// the angle in turns in double (pos times a frequency keeps no fraction in 24 bits at far positions), its fraction in float.
+// Head widths, row strides or addresses that do not allow float4 run the same steps with one warp a head, pairs of floats.
+// dgain: each CTA leaves its sums in the caller's scratch, a second launch adds them in a fixed order.
+#include <math.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace {
+
+constexpr int WARPS = 8, THREADS = 32 * WARPS;
+constexpr int MAX_PARTS = FML_QK_NORM_ROPE_PARTS;   // CTAs of a backward launch, one partial sum each
+constexpr int MAX_D = 256;
+
+struct Side {          // queries or keys
+  const float* x;
+  const float* dy;     // backward
+  float* out;          // y, or dx
+  long long ldx, ldy, ldo;
+  const float* gain;
+  int heads;
+};
+struct Params {
+  Side s[2];
+  const int* pos;
+  float* parts;        // [CTA][2][d], or NULL when no gain gradient is wanted
+  long long rows;
+  int seq_len, d, rot, interleaved, accumulate;
+  int rows_cta;        // rows of a CTA's step
+  double kexp;         // -2 log2(base) / rot
+  float eps;
+};
+
+// cosines and sines of rows [r0, r0 + n) into tab[row][rot / 2] and tab2[row][rot / 2]
+__device__ __forceinline__ void angles(const Params& p, long long r0, int n, float* cosv, float* sinv) {
+  const int half = p.rot >> 1;
+  for (int i = threadIdx.x; i < n * half; i += THREADS) {
+    const int r = i / half, j = i - r * half;
+    const long long row = r0 + r;
+    const double pos = p.pos ? (double)p.pos[row] : (double)(p.seq_len > 0 ? row % p.seq_len : row);
+    const double turns = pos * (exp2(p.kexp * j) * 0.15915494309189533577);
+    float s, c;
+    sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
+    cosv[i] = c;
+    sinv[i] = s;
+  }
+}
+
+template <int LPH>
+__device__ __forceinline__ float head_sum(float v) {
+#pragma unroll
+  for (int o = LPH / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// the lane's eight elements turned by +angle (sign = 1) or back (sign = -1)
+__device__ __forceinline__ void turn8(float* z, const float* c, const float* s, float sign, int interleaved) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int ia = interleaved ? 2 * i : i, ib = interleaved ? 2 * i + 1 : i + 4;
+    const float a = z[ia], b = z[ib], sn = sign * s[i];
+    z[ia] = a * c[i] - b * sn;
+    z[ib] = a * sn + b * c[i];
+  }
+}
+
+template <int LPH, bool BWD, bool INTER>
+__global__ void __launch_bounds__(THREADS) qk_vec_kernel(const Params p) {
+  extern __shared__ float sm[];
+  constexpr int HPW = 32 / LPH;                       // heads of a warp's item
+  constexpr int U = BWD ? 2 : 4;                      // items whose loads go out together
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int u = lane % LPH, sub = lane / LPH;
+  const int half = p.rot >> 1, d = p.d;
+  float* cosv = sm;
+  float* sinv = sm + p.rows_cta * half;
+  const int total = p.s[0].heads + p.s[1].heads;
+  const int groups = (total + HPW - 1) / HPW;
+  // the lane's place in a head: e0, e1 (four elements each); a rotated unit takes both halves of its pairs
+  const bool active = u < (d >> 3);
+  const bool turned = u < (p.rot >> 3);
+  const int e0 = turned ? 4 * u : p.rot + 4 * (u - (p.rot >> 3));
+  const int e1 = turned ? 4 * u + half : e0 + ((d - p.rot) >> 1);
+  float gain[2][8], dg[2][8];
+#pragma unroll
+  for (int t = 0; t < 2; t++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      gain[t][i] = active && p.s[t].gain ? p.s[t].gain[(i < 4 ? e0 : e1) + (i & 3)] : 1.f;
+      dg[t][i] = 0.f;
+    }
+  const float inv_d = 1.f / (float)d;
+  const long long steps = (p.rows + p.rows_cta - 1) / p.rows_cta;
+  for (long long st = blockIdx.x; st < steps; st += gridDim.x) {
+    const long long r0 = st * p.rows_cta;
+    const int n = (int)min((long long)p.rows_cta, p.rows - r0);
+    __syncthreads();                                  // the table of the step before has been read
+    angles(p, r0, n, cosv, sinv);
+    __syncthreads();
+    const int items = n * groups;
+    for (int it0 = warp; it0 < items; it0 += WARPS * U) {
+      float x[U][8], dy[BWD ? U : 1][8];
+#pragma unroll
+      for (int k = 0; k < U; k++) {
+        const int it = it0 + k * WARPS;
+        const int r = it / groups, head = (it - r * groups) * HPW + sub;
+        const bool on = it < items && active && head < total;
+        const bool key = head >= p.s[0].heads;
+        const Side& s = p.s[key ? 1 : 0];
+        const int hh = key ? head - p.s[0].heads : head;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+        if (on) {
+          const float* src = s.x + (r0 + r) * s.ldx + (long long)hh * d;
+          a = *reinterpret_cast<const float4*>(src + e0);
+          b = *reinterpret_cast<const float4*>(src + e1);
+        }
+        reinterpret_cast<float4*>(x[k])[0] = a;
+        reinterpret_cast<float4*>(x[k])[1] = b;
+        if (BWD) {
+          a = b = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (on) {
+            const float* src = s.dy + (r0 + r) * s.ldy + (long long)hh * d;
+            a = *reinterpret_cast<const float4*>(src + e0);
+            b = *reinterpret_cast<const float4*>(src + e1);
+          }
+          reinterpret_cast<float4*>(dy[k])[0] = a;
+          reinterpret_cast<float4*>(dy[k])[1] = b;
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < U; k++) {
+        const int it = it0 + k * WARPS;
+        if (it >= items) break;                       // the same for the whole warp
+        const int r = it / groups, head = (it - r * groups) * HPW + sub;
+        const bool on = active && head < total;
+        const bool key = head >= p.s[0].heads;
+        const Side& s = p.s[key ? 1 : 0];
+        const int hh = key ? head - p.s[0].heads : head;
+        float c[4], sn[4];
+        if (turned) {
+          if (INTER) {
+            *reinterpret_cast<float2*>(c) = *reinterpret_cast<const float2*>(cosv + r * half + 2 * u);
+            *reinterpret_cast<float2*>(c + 2) = *reinterpret_cast<const float2*>(cosv + r * half + (half >> 1) + 2 * u);
+            *reinterpret_cast<float2*>(sn) = *reinterpret_cast<const float2*>(sinv + r * half + 2 * u);
+            *reinterpret_cast<float2*>(sn + 2) = *reinterpret_cast<const float2*>(sinv + r * half + (half >> 1) + 2 * u);
+          } else {
+            *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(cosv + r * half + 4 * u);
+            *reinterpret_cast<float4*>(sn) = *reinterpret_cast<const float4*>(sinv + r * half + 4 * u);
+          }
+        }
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) ss = fmaf(x[k][i], x[k][i], ss);
+        const float rstd = 1.f / sqrtf(fmaf(head_sum<LPH>(ss), inv_d, p.eps));
+        float z[8];
+        if (!BWD) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) z[i] = x[k][i] * rstd * (key ? gain[1][i] : gain[0][i]);
+          if (turned) turn8(z, c, sn, 1.f, INTER);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; i++) z[i] = dy[k][i];
+          if (turned) turn8(z, c, sn, -1.f, INTER);
+          float dot = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            const float xh = x[k][i] * rstd, dgi = z[i] * xh;
+            if (key) dg[1][i] += dgi; else dg[0][i] += dgi;
+            z[i] *= key ? gain[1][i] : gain[0][i];
+            dot = fmaf(z[i], xh, dot);
+            x[k][i] = xh;
+          }
+          dot = head_sum<LPH>(dot) * inv_d;
+#pragma unroll
+          for (int i = 0; i < 8; i++) z[i] = rstd * (z[i] - x[k][i] * dot);
+        }
+        if (on) {
+          float* dst = s.out + (r0 + r) * s.ldo + (long long)hh * d;
+          float4 a = reinterpret_cast<float4*>(z)[0], b = reinterpret_cast<float4*>(z)[1];
+          if (BWD && p.accumulate) {
+            const float4 oa = *reinterpret_cast<const float4*>(dst + e0), ob = *reinterpret_cast<const float4*>(dst + e1);
+            a.x += oa.x; a.y += oa.y; a.z += oa.z; a.w += oa.w;
+            b.x += ob.x; b.y += ob.y; b.z += ob.z; b.w += ob.w;
+          }
+          *reinterpret_cast<float4*>(dst + e0) = a;
+          *reinterpret_cast<float4*>(dst + e1) = b;
+        }
+      }
+    }
+  }
+  if (!BWD || !p.parts) return;
+  // the CTA's sums: over the warp's heads, then over the warps, in a fixed order
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < 2; t++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      float v = dg[t][i];
+#pragma unroll
+      for (int o = LPH; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (sub == 0 && active) sm[(warp * 2 + t) * d + (i < 4 ? e0 : e1) + (i & 3)] = v;
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * d; i += THREADS) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) v += sm[w * 2 * d + i];
+    p.parts[(long long)blockIdx.x * 2 * d + i] = v;
+  }
+}
+
+// One warp a head, its elements as pairs: the rotated ones, then neighbours of the rest (the last may be half a pair).
+template <bool BWD>
+__global__ void __launch_bounds__(THREADS) qk_pair_kernel(const Params p) {
+  extern __shared__ float sm[];
+  constexpr int SLOTS = MAX_D / 64;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int half = p.rot >> 1, d = p.d;
+  float* cosv = sm;
+  float* sinv = sm + p.rows_cta * half;
+  const int total = p.s[0].heads + p.s[1].heads;
+  int ea[SLOTS], eb[SLOTS];                            // elements of the lane's pairs, -1: none
+  float dg[2][SLOTS][2];
+#pragma unroll
+  for (int j = 0; j < SLOTS; j++) {
+    const int q = lane + 32 * j;
+    if (q < half) {
+      ea[j] = p.interleaved ? 2 * q : q;
+      eb[j] = p.interleaved ? 2 * q + 1 : q + half;
+    } else {
+      const int e = p.rot + 2 * (q - half);
+      ea[j] = e < d ? e : -1;
+      eb[j] = e + 1 < d ? e + 1 : -1;
+    }
+    dg[0][j][0] = dg[0][j][1] = dg[1][j][0] = dg[1][j][1] = 0.f;
+  }
+  const float inv_d = 1.f / (float)d;
+  const long long steps = (p.rows + p.rows_cta - 1) / p.rows_cta;
+  for (long long st = blockIdx.x; st < steps; st += gridDim.x) {
+    const long long r0 = st * p.rows_cta;
+    const int n = (int)min((long long)p.rows_cta, p.rows - r0);
+    __syncthreads();
+    angles(p, r0, n, cosv, sinv);
+    __syncthreads();
+    for (int it = warp; it < n * total; it += WARPS) {
+      const int r = it / total, head = it - r * total;
+      const int key = head >= p.s[0].heads;
+      const Side& s = p.s[key];
+      const long long h0 = (long long)(key ? head - p.s[0].heads : head) * d;
+      const float* src = s.x + (r0 + r) * s.ldx + h0;
+      float xa[SLOTS], xb[SLOTS], ya[SLOTS], yb[SLOTS];
+#pragma unroll
+      for (int j = 0; j < SLOTS; j++) {
+        xa[j] = ea[j] >= 0 ? src[ea[j]] : 0.f;
+        xb[j] = eb[j] >= 0 ? src[eb[j]] : 0.f;
+      }
+      if (BWD) {
+        const float* dsrc = s.dy + (r0 + r) * s.ldy + h0;
+#pragma unroll
+        for (int j = 0; j < SLOTS; j++) {
+          ya[j] = ea[j] >= 0 ? dsrc[ea[j]] : 0.f;
+          yb[j] = eb[j] >= 0 ? dsrc[eb[j]] : 0.f;
+        }
+      }
+      float ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < SLOTS; j++) ss = fmaf(xa[j], xa[j], fmaf(xb[j], xb[j], ss));
+      const float rstd = 1.f / sqrtf(fmaf(head_sum<32>(ss), inv_d, p.eps));
+      float dot = 0.f;
+#pragma unroll
+      for (int j = 0; j < SLOTS; j++) {
+        const int q = lane + 32 * j;
+        const float c = q < half ? cosv[r * half + q] : 1.f, sn = q < half ? sinv[r * half + q] : 0.f;
+        const float ga = s.gain && ea[j] >= 0 ? s.gain[ea[j]] : 1.f, gb = s.gain && eb[j] >= 0 ? s.gain[eb[j]] : 1.f;
+        xa[j] *= rstd;
+        xb[j] *= rstd;
+        if (!BWD) {
+          const float za = xa[j] * ga, zb = xb[j] * gb;
+          ya[j] = q < half ? za * c - zb * sn : za;
+          yb[j] = q < half ? za * sn + zb * c : zb;
+        } else {
+          float za = q < half ? ya[j] * c + yb[j] * sn : ya[j], zb = q < half ? yb[j] * c - ya[j] * sn : yb[j];
+          dg[0][j][0] += key ? 0.f : za * xa[j];
+          dg[0][j][1] += key ? 0.f : zb * xb[j];
+          dg[1][j][0] += key ? za * xa[j] : 0.f;
+          dg[1][j][1] += key ? zb * xb[j] : 0.f;
+          za *= ga;
+          zb *= gb;
+          dot = fmaf(za, xa[j], fmaf(zb, xb[j], dot));
+          ya[j] = za;
+          yb[j] = zb;
+        }
+      }
+      if (BWD) {
+        dot = head_sum<32>(dot) * inv_d;
+#pragma unroll
+        for (int j = 0; j < SLOTS; j++) {
+          ya[j] = rstd * (ya[j] - xa[j] * dot);
+          yb[j] = rstd * (yb[j] - xb[j] * dot);
+        }
+      }
+      float* dst = s.out + (r0 + r) * s.ldo + h0;
+#pragma unroll
+      for (int j = 0; j < SLOTS; j++) {
+        if (ea[j] >= 0) dst[ea[j]] = BWD && p.accumulate ? dst[ea[j]] + ya[j] : ya[j];
+        if (eb[j] >= 0) dst[eb[j]] = BWD && p.accumulate ? dst[eb[j]] + yb[j] : yb[j];
+      }
+    }
+  }
+  if (!BWD || !p.parts) return;
+  __syncthreads();
+#pragma unroll
+  for (int t = 0; t < 2; t++)
+#pragma unroll
+    for (int j = 0; j < SLOTS; j++) {
+      if (ea[j] >= 0) sm[(warp * 2 + t) * d + ea[j]] = dg[t][j][0];
+      if (eb[j] >= 0) sm[(warp * 2 + t) * d + eb[j]] = dg[t][j][1];
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * d; i += THREADS) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) v += sm[w * 2 * d + i];
+    p.parts[(long long)blockIdx.x * 2 * d + i] = v;
+  }
+}
+
+// dgain += the CTAs' sums, 32 columns a block, in a fixed order
+__global__ void __launch_bounds__(THREADS) qk_gain_kernel(const float* __restrict__ parts, int n_parts, int d, float* dgain_q, float* dgain_k) {
+  __shared__ float red[WARPS][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
+  float v = 0.f;
+  if (i < 2 * d) {
+#pragma unroll 8
+    for (int c = warp; c < n_parts; c += WARPS) v += parts[(long long)c * 2 * d + i];
+  }
+  red[warp][lane] = v;
+  __syncthreads();
+  if (warp != 0 || i >= 2 * d) return;
+  for (int w = 1; w < WARPS; w++) v += red[w][lane];
+  float* dst = i < d ? dgain_q : dgain_k;
+  if (dst) dst[i < d ? i : i - d] += v;
+}
+
+bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Whether two row-strided slices share an element.  Slices of one row stride are compared column by column, so the
+// parts of a fused projection are told apart; others by their ranges.
+bool clash(const float* a, long long lda, long long wa, const float* b, long long ldb, long long wb, long long rows) {
+  if (!a || !b || rows == 0 || wa == 0 || wb == 0) return false;
+  const uintptr_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
+  if (pa + 4 * ((rows - 1) * lda + wa) <= pb || pb + 4 * ((rows - 1) * ldb + wb) <= pa) return false;
+  if (lda != ldb || (pa & 3) != (pb & 3)) return true;
+  const long long off = ((long long)(pb - pa) / 4 % lda + lda) % lda;   // b's first column, counted from a's
+  return off < wa || off + wb > lda;
+}
+bool same(const float* a, long long lda, const float* b, long long ldb) { return a == b && lda == ldb; }
+
+int32_t check(fml_ctx* ctx, const Params& p, double base) {
+  FML_REQUIRE(ctx, p.rows >= 0 && p.d >= 1 && p.d <= MAX_D, "fml_qk_norm_rope: d_head must be 1 .. 256");
+  FML_REQUIRE(ctx, p.s[0].heads >= 1 && p.s[1].heads >= 0 && p.s[0].heads <= (1 << 20) && p.s[1].heads <= (1 << 20), "fml_qk_norm_rope: bad number of heads");
+  FML_REQUIRE(ctx, p.rot >= 0 && p.rot <= p.d && p.rot % 2 == 0, "fml_qk_norm_rope: rot_dim must be even, 0 .. d_head");
+  FML_REQUIRE(ctx, p.rot == 0 || (base > 0 && isfinite(base)), "fml_qk_norm_rope: base must be positive");
+  FML_REQUIRE(ctx, p.eps > 0 && isfinite(p.eps), "fml_qk_norm_rope: eps must be positive");
+  FML_REQUIRE(ctx, p.seq_len >= 0, "fml_qk_norm_rope: bad seq_len");
+  for (int t = 0; t < 2; t++) {
+    const Side& s = p.s[t];
+    if (s.heads == 0) continue;
+    FML_REQUIRE(ctx, s.x && s.out && ((reinterpret_cast<uintptr_t>(s.x) | reinterpret_cast<uintptr_t>(s.out) | reinterpret_cast<uintptr_t>(s.dy)) & 3) == 0,
+                "fml_qk_norm_rope: missing or misaligned buffer");
+    const long long w = (long long)s.heads * p.d;
+    FML_REQUIRE(ctx, s.ldx >= w && s.ldo >= w && (!s.dy || s.ldy >= w), "fml_qk_norm_rope: a row stride is shorter than the heads");
+  }
+  // an output may take the place of its own input; anything else that it shares with another buffer would be read after
+  // it was overwritten
+  for (int t = 0; t < 2; t++) {
+    const Side& s = p.s[t];
+    const long long w = (long long)s.heads * p.d;
+    for (int o = 0; o < 2; o++) {
+      const Side& q = p.s[o];
+      const long long wq = (long long)q.heads * p.d;
+      const bool x_ok = o == t && same(s.out, s.ldo, q.x, q.ldx), dy_ok = o == t && same(s.out, s.ldo, q.dy, q.ldy) && !p.accumulate;
+      FML_REQUIRE(ctx, x_ok || !clash(s.out, s.ldo, w, q.x, q.ldx, wq, p.rows), "fml_qk_norm_rope: an output overlaps an input");
+      FML_REQUIRE(ctx, dy_ok || !clash(s.out, s.ldo, w, q.dy, q.ldy, wq, p.rows), "fml_qk_norm_rope: an output overlaps an input");
+    }
+  }
+  FML_REQUIRE(ctx, !clash(p.s[0].out, p.s[0].ldo, (long long)p.s[0].heads * p.d, p.s[1].out, p.s[1].ldo, (long long)p.s[1].heads * p.d, p.rows),
+              "fml_qk_norm_rope: the outputs overlap");
+  return FML_OK;
+}
+
+bool can_vec(const Params& p) {
+  if (p.d % 8 || p.rot % 8) return false;   // rest of the head: a multiple of 8 too
+  for (int t = 0; t < 2; t++) {
+    const Side& s = p.s[t];
+    if (s.heads == 0) continue;
+    if (!al16(s.x) || !al16(s.out) || s.ldx % 4 || s.ldo % 4 || (s.dy && (!al16(s.dy) || s.ldy % 4))) return false;
+  }
+  return true;
+}
+
+template <int LPH, bool BWD>
+void launch_vec(const Params& p, int grid, size_t smem, cudaStream_t s) {
+  if (p.interleaved) qk_vec_kernel<LPH, BWD, true><<<grid, THREADS, smem, s>>>(p);
+  else qk_vec_kernel<LPH, BWD, false><<<grid, THREADS, smem, s>>>(p);
+}
+
+template <bool BWD>
+int32_t launch(fml_ctx* ctx, Params& p, int* grid_out) {
+  const bool vec = can_vec(p);
+  const int lph = p.d <= 32 ? 4 : p.d <= 64 ? 8 : p.d <= 128 ? 16 : 32;
+  const int total = p.s[0].heads + p.s[1].heads;
+  const int items = vec ? (total + 32 / lph - 1) / (32 / lph) : total;   // a row's
+  // rows of a CTA's step: 64 items give every warp eight, and the angles are formed by all threads; fewer rows where
+  // that would leave SMs without work
+  long long rc = std::max(1, std::min(16, 64 / items));
+  while (rc > 1 && (p.rows + rc - 1) / rc < 2ll * ctx->sm_count) rc >>= 1;
+  p.rows_cta = (int)rc;
+  const long long steps = (p.rows + rc - 1) / rc;
+  const int grid = (int)std::min<long long>(steps, BWD ? std::min(MAX_PARTS, 4 * ctx->sm_count) : 8ll * ctx->sm_count);
+  const size_t smem = std::max<size_t>((size_t)rc * p.rot * 4, BWD ? (size_t)WARPS * 2 * p.d * 4 : 0);   // at most 16 KB
+  if (!vec) qk_pair_kernel<BWD><<<grid, THREADS, smem, ctx->stream>>>(p);
+  else if (lph == 4) launch_vec<4, BWD>(p, grid, smem, ctx->stream);
+  else if (lph == 8) launch_vec<8, BWD>(p, grid, smem, ctx->stream);
+  else if (lph == 16) launch_vec<16, BWD>(p, grid, smem, ctx->stream);
+  else launch_vec<32, BWD>(p, grid, smem, ctx->stream);
+  FML_LAUNCH_CHECK(ctx, "qk_norm_rope kernel");
+  *grid_out = grid;
+  return FML_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t fml_qk_norm_rope_fwd(fml_ctx* ctx, const float* q, int64_t ld_q, float* q_out, int64_t ld_q_out, int32_t heads_q, const float* k,
+                             int64_t ld_k, float* k_out, int64_t ld_k_out, int32_t heads_k, int64_t rows, int32_t d_head,
+                             const float* gain_q, const float* gain_k, const int32_t* positions, int32_t seq_len, int32_t rot_dim,
+                             int32_t interleaved, double base, float eps) {
+  FML_REQUIRE(ctx, ctx, "fml_qk_norm_rope_fwd: no context");
+  FML_ENTER(ctx);
+  Params p = {};
+  p.s[0] = {q, nullptr, q_out, ld_q, 0, ld_q_out, gain_q, heads_q};
+  p.s[1] = {k, nullptr, k_out, ld_k, 0, ld_k_out, gain_k, heads_k};
+  p.pos = positions; p.rows = rows; p.seq_len = seq_len; p.d = d_head; p.rot = rot_dim; p.interleaved = interleaved != 0; p.eps = eps;
+  int32_t rc = check(ctx, p, base);
+  if (rc || rows == 0) return rc;
+  p.kexp = rot_dim ? -2.0 * log2(base) / rot_dim : 0.0;
+  int grid;
+  return launch<false>(ctx, p, &grid);
+}
+
+int32_t fml_qk_norm_rope_bwd(fml_ctx* ctx, const float* q, int64_t ld_q, const float* dq_out, int64_t ld_dq_out, float* dq, int64_t ld_dq,
+                             int32_t heads_q, const float* k, int64_t ld_k, const float* dk_out, int64_t ld_dk_out, float* dk,
+                             int64_t ld_dk, int32_t heads_k, int64_t rows, int32_t d_head, const float* gain_q, const float* gain_k,
+                             float* dgain_q, float* dgain_k, const int32_t* positions, int32_t seq_len, int32_t rot_dim,
+                             int32_t interleaved, double base, float eps, int32_t accumulate, float* scratch) {
+  FML_REQUIRE(ctx, ctx, "fml_qk_norm_rope_bwd: no context");
+  FML_ENTER(ctx);
+  Params p = {};
+  p.s[0] = {q, dq_out, dq, ld_q, ld_dq_out, ld_dq, gain_q, heads_q};
+  p.s[1] = {k, dk_out, dk, ld_k, ld_dk_out, ld_dk, gain_k, heads_k};
+  p.pos = positions; p.rows = rows; p.seq_len = seq_len; p.d = d_head; p.rot = rot_dim; p.interleaved = interleaved != 0; p.eps = eps;
+  p.accumulate = accumulate != 0;
+  int32_t rc = check(ctx, p, base);
+  if (rc) return rc;
+  FML_REQUIRE(ctx, dq_out && (heads_k == 0 || dk_out), "fml_qk_norm_rope_bwd: missing gradient");
+  FML_REQUIRE(ctx, (!dgain_q || gain_q) && (!dgain_k || (gain_k && heads_k)), "fml_qk_norm_rope_bwd: the gradient of a gain that is not there");
+  FML_REQUIRE(ctx, !(dgain_q || dgain_k) || scratch, "fml_qk_norm_rope_bwd: gain gradients need the scratch buffer");
+  if (rows == 0) return FML_OK;
+  p.kexp = rot_dim ? -2.0 * log2(base) / rot_dim : 0.0;
+  p.parts = dgain_q || dgain_k ? scratch : nullptr;
+  int grid;
+  rc = launch<true>(ctx, p, &grid);
+  if (rc || !p.parts) return rc;
+  qk_gain_kernel<<<(2 * d_head + 31) / 32, THREADS, 0, ctx->stream>>>(scratch, grid, d_head, dgain_q, dgain_k);
+  FML_LAUNCH_CHECK(ctx, "qk_gain_kernel");
+  return FML_OK;
+}
+
+}  // extern "C"

@@ -650,12 +650,17 @@ class MultiHeadAttention(Layer):
 
     The per-head Wq, Wk, Wv [dModel x dK] live side by side in ONE matrix Wqkv
     [dModel x 3*dModel] laid out [Q heads | K heads | V heads], so columns h*dK..(h+1)*dK of each
-    third are exactly head h's reference matrix and X.Wqkv is a single product."""
+    third are exactly head h's reference matrix and X.Wqkv is a single product.
+
+    Extension: qkNorm=True norms every query and key head (gains `gainQ`, `gainK` of dModel/numHeads elements, ones at the
+    start, two more parameters) and turns its first `rotaryDim` columns by position (None: all, 0: none; `rotaryBase`,
+    `rotaryInterleaved` as in T.QKNorm) before the scores, in one launch."""
 
     name = "multi_head_attention"
 
     def __init__(self, dModel: int, numHeads: int, seq_len: Optional[int] = None, causal: bool = False, seed: int = 0,
-                 head_weights=None, Wo=None, precision: int = -1):
+                 head_weights=None, Wo=None, precision: int = -1, qkNorm: bool = False, rotaryDim: Optional[int] = None,
+                 rotaryBase: float = 10000.0, rotaryInterleaved: bool = False):
         """Argument order of the reference: MultiHeadAttention(dModel, numHeads) (multiHeadAttentionLayer.dart:33)."""
         super().__init__()
         if numHeads <= 0 or dModel % numHeads != 0:
@@ -663,7 +668,8 @@ class MultiHeadAttention(Layer):
         self.numHeads, self.dModel, self.dK = numHeads, dModel, dModel // numHeads
         self.seq_len, self.causal, self.seed, self.precision = seq_len, causal, seed, precision
         self._heads0, self._wo0 = head_weights, Wo
-        self.Wqkv = self.Wo = None
+        self.qkNorm, self.rotaryDim, self.rotaryBase, self.rotaryInterleaved = qkNorm, rotaryDim, rotaryBase, rotaryInterleaved
+        self.Wqkv = self.Wo = self.gainQ = self.gainK = None
         self.lastAttentionWeights = None
 
     @staticmethod
@@ -679,7 +685,16 @@ class MultiHeadAttention(Layer):
 
     @property
     def parameters(self):
-        return [self.Wqkv, self.Wo]
+        return [self.Wqkv, self.Wo] + self._gains
+
+    @property
+    def _gains(self):
+        return [self.gainQ, self.gainK] if self.qkNorm else []
+
+    def _qk_norm(self):
+        if not self.qkNorm:
+            return None
+        return T.QKNorm(self.gainQ, self.gainK, None, self.rotaryDim, self.rotaryBase, self.rotaryInterleaved)
 
     def build(self, x: Tensor):
         d = self.dModel
@@ -690,13 +705,15 @@ class MultiHeadAttention(Layer):
             wqkv = synth.uniform(self.seed, 0, (d, 3 * d), -a, a)
         wo = self._wo0 if self._wo0 is not None else synth.uniform(self.seed, 1, (d, d), -a, a)
         self.Wqkv, self.Wo = Tensor(np.ascontiguousarray(wqkv, dtype=np.float32), x.ctx), Tensor(wo, x.ctx)
+        if self.qkNorm:
+            self.gainQ, self.gainK = (Tensor(np.ones(self.dK, dtype=np.float32), x.ctx) for _ in range(2))
         super().build(x)
 
     def forward(self, x: Tensor) -> Tensor:
         S = self.seq_len or x.shape[0]
         n_seq = x.shape[0] // S
         qkv = T.denseMatrix(x, self.Wqkv, None, None, self.precision)
-        o = T.attentionCore(qkv, n_seq, S, self.numHeads, self.dK, self.causal, self.precision)
+        o = T.attentionCore(qkv, n_seq, S, self.numHeads, self.dK, self.causal, self.precision, self._qk_norm())
         self.lastAttentionWeights = o.attention_weights
         return T.denseMatrix(o, self.Wo, None, None, self.precision)
 
@@ -729,10 +746,10 @@ class TransformerEncoderBlock(Layer):
     name = "transformer_encoder_block"
 
     def __init__(self, dModel: int, numHeads: int, dff: int, seq_len=None, causal=False, seed: int = 0, params=None,
-                 precision: int = -1):
+                 precision: int = -1, qkNorm: bool = False):
         super().__init__()
         p = params or {}
-        self.attention = MultiHeadAttention(dModel, numHeads, seq_len, causal, seed, p.get("heads"), p.get("Wo"), precision)
+        self.attention = MultiHeadAttention(dModel, numHeads, seq_len, causal, seed, p.get("heads"), p.get("Wo"), precision, qkNorm)
         self.norm1, self.norm2 = LayerNormalization(), LayerNormalization()
         self.ffn1 = DenseLayerMatrix(dff, "relu", seed + 1, p.get("W1"), p.get("b1"), precision)
         self.ffn2 = DenseLayerMatrix(dModel, None, seed + 2, p.get("W2"), p.get("b2"), precision)

@@ -175,6 +175,33 @@ class DenseFwdBwdHost:
         return self.h_out
 
 
+def qk_norm_rope_scratch(d_head: int) -> int:
+    """Floats of the scratch buffer that the gain gradients of `qk_norm_rope_backward` go through."""
+    return _lib.QK_NORM_ROPE_PARTS * 2 * d_head
+
+
+def qk_norm_rope_forward(ctx, q, k, q_out, k_out, rows, heads_q, heads_k, d_head, gain_q=None, gain_k=None, positions=None, seq_len=0,
+                         rot_dim=None, interleaved=False, base=10000.0, eps=1e-6, ld_q=None, ld_k=None, ld_q_out=None, ld_k_out=None):
+    """Norm of every query and key head, its gain, and the rotation by position, in one launch (`fml_qk_norm_rope_fwd`).
+    Row strides default to rows that lie end to end; rot_dim defaults to the whole head; k may be None with heads_k = 0."""
+    wq, wk = heads_q * d_head, heads_k * d_head
+    ctx.call("fml_qk_norm_rope_fwd", q, ld_q or wq, q_out, ld_q_out or wq, heads_q, k, ld_k or wk, k_out, ld_k_out or wk, heads_k, rows, d_head,
+             gain_q, gain_k, positions, seq_len, d_head if rot_dim is None else rot_dim, 1 if interleaved else 0, base, eps)
+
+
+def qk_norm_rope_backward(ctx, q, k, dq_out, dk_out, dq, dk, rows, heads_q, heads_k, d_head, gain_q=None, gain_k=None, dgain_q=None,
+                          dgain_k=None, positions=None, seq_len=0, rot_dim=None, interleaved=False, base=10000.0, eps=1e-6, ld_q=None,
+                          ld_k=None, ld_dq_out=None, ld_dk_out=None, ld_dq=None, ld_dk=None, accumulate=False, scratch=None):
+    """Gradients of `qk_norm_rope_forward` (`fml_qk_norm_rope_bwd`); dgain_q and dgain_k are added to, through `scratch` of
+    `qk_norm_rope_scratch(d_head)` floats."""
+    wq, wk = heads_q * d_head, heads_k * d_head
+    if scratch is not None and scratch.size < qk_norm_rope_scratch(d_head):
+        raise ValueError(f"qk_norm_rope_backward: the scratch buffer needs {qk_norm_rope_scratch(d_head)} floats")
+    ctx.call("fml_qk_norm_rope_bwd", q, ld_q or wq, dq_out, ld_dq_out or wq, dq, ld_dq or wq, heads_q, k, ld_k or wk, dk_out, ld_dk_out or wk, dk,
+             ld_dk or wk, heads_k, rows, d_head, gain_q, gain_k, dgain_q, dgain_k, positions, seq_len, d_head if rot_dim is None else rot_dim,
+             1 if interleaved else 0, base, eps, 1 if accumulate else 0, scratch, launches=2 if dgain_q is not None or dgain_k is not None else 1)
+
+
 class AdamWPlan:
     """AdamW (lib/optimizers/adamw.dart:82-89) over a list of tensors in one launch (`fml_adamw_plan_*`).  `w` and `g` are
     lists of device arrays, `m` and `v` the two state buffers of `state_floats(sizes, stateBits)` floats, zeroed before the

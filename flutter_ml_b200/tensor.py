@@ -18,7 +18,7 @@ from typing import List, Optional, Sequence
 
 import numpy as np
 
-from . import _lib
+from . import _lib, ops
 from ._lib import ACT_BY_NAME, Context, DeviceArray
 
 _default_ctx: Optional[Context] = None
@@ -410,7 +410,67 @@ def layerNorm(x: Tensor, gamma: Tensor, beta: Tensor, epsilon: float = 1e-5, res
     return out
 
 
-def _attentionFused(qkv: Tensor, q, k, v, Bn, S, H, dk, causal, scale):
+class QKNorm:
+    """What the norm of queries and keys with the position rotation needs besides its inputs: the gains (Tensors of d_head
+    elements, or None for ones), the positions (an int32 device array with one entry a row, or None: row mod seq_len), how
+    many columns of a head are turned (None: all), the base of the frequencies, and which pairs."""
+
+    def __init__(self, gain_q: Optional[Tensor] = None, gain_k: Optional[Tensor] = None, positions: Optional[DeviceArray] = None,
+                 rot_dim: Optional[int] = None, base: float = 10000.0, interleaved: bool = False, eps: float = 1e-6):
+        self.gain_q, self.gain_k, self.positions = gain_q, gain_k, positions
+        self.rot_dim, self.base, self.interleaved, self.eps = rot_dim, base, interleaved, eps
+
+    @property
+    def inputs(self):
+        return [g for g in (self.gain_q, self.gain_k) if g is not None]
+
+    def _options(self, rows, seq_len, ld):
+        if self.positions is not None and (self.positions.dtype != np.int32 or self.positions.size < rows):
+            raise ValueError("QKNorm: positions must be int32, one for each row")
+        return dict(gain_q=self.gain_q.value if self.gain_q is not None else None, gain_k=self.gain_k.value if self.gain_k is not None else None,
+                    positions=self.positions, seq_len=seq_len, rot_dim=self.rot_dim, interleaved=self.interleaved, base=self.base,
+                    eps=self.eps, ld_q=ld, ld_k=ld)
+
+    def forward(self, ctx, x, out, rows, seq_len, heads_q, heads_k, d_head, ld, ld_out):
+        """x, out: buffers with the queries in their first heads_q * d_head columns and the keys behind them."""
+        d = heads_q * d_head
+        ops.qk_norm_rope_forward(ctx, x, x.view(d, ()), out, out.view(d, ()), rows, heads_q, heads_k, d_head, ld_q_out=ld_out, ld_k_out=ld_out,
+                                 **self._options(rows, seq_len, ld))
+
+    def backward(self, ctx, x, dout, dx, rows, seq_len, heads_q, heads_k, d_head, ld, ld_dout, accumulate):
+        d = heads_q * d_head
+        for g in self.inputs:
+            if g.grad is None:
+                g.zeroGrad()
+        scratch = ctx.empty(ops.qk_norm_rope_scratch(d_head)) if self.inputs else None
+        ops.qk_norm_rope_backward(ctx, x, x.view(d, ()), dout, dout.view(d, ()), dx, dx.view(d, ()), rows, heads_q, heads_k, d_head,
+                                  dgain_q=self.gain_q.grad if self.gain_q is not None else None,
+                                  dgain_k=self.gain_k.grad if self.gain_k is not None else None, ld_dq_out=ld_dout, ld_dk_out=ld_dout, ld_dq=ld,
+                                  ld_dk=ld, accumulate=accumulate, scratch=scratch, **self._options(rows, seq_len, ld))
+
+
+def qkNormRope(x: Tensor, heads_q: int, heads_k: int, d_head: int, norm: Optional[QKNorm] = None, seq_len: int = 0) -> Tensor:
+    """Queries and keys in the first (heads_q + heads_k) * d_head columns of x (a fused projection; what lies behind them,
+    values for instance, is not read) -> the normed and turned ones, [rows x (heads_q + heads_k) * d_head].  Extension: it
+    stands between the projections and the attention of lib/layertypes/singleHeadAttentionLayer.dart:77-86."""
+    ctx, norm = x.ctx, norm or QKNorm()
+    R, W = x.shape
+    C = (heads_q + heads_k) * d_head
+    if W < C:
+        raise ValueError(f"qkNormRope: {heads_q} + {heads_k} heads of {d_head} do not fit {W} columns")
+    out = Tensor(ctx.empty(R, C), ctx)
+    norm.forward(ctx, x.value, out.value, R, seq_len, heads_q, heads_k, d_head, W, C)
+
+    def bw():
+        g, acc = x._grad_target()
+        if not acc and W > C:
+            ctx.zero(g)          # the columns that were not read
+        norm.backward(ctx, x.value, out.grad, g, R, seq_len, heads_q, heads_k, d_head, W, C, acc)
+    out.creator = Node([x] + norm.inputs, bw, "qk_norm_rope", 8 * R * C)
+    return out
+
+
+def _attentionFused(qkv: Tensor, q, k, v, Bn, S, H, dk, causal, scale, qk_norm=None):
     """fml_attention_fwd / fml_attention_bwd: the score matrices stay on chip in the forward pass; the backward
     pass rebuilds the probabilities from the saved row statistics and writes only P and dS once."""
     import ctypes
@@ -428,33 +488,50 @@ def _attentionFused(qkv: Tensor, q, k, v, Bn, S, H, dk, causal, scale):
     global fused_attention_calls
     fused_attention_calls += 1
 
-    def bw():
+    def bw(_normed=q):  # with qk_norm, q and k live in a buffer of their own that only this closure keeps
         g, acc = qkv._grad_target()
         scratch = ctx.empty(Bn * H * S)
-        ctx.check(ctx.lib.fml_attention_bwd(ctx.h, ctypes.byref(desc), out.grad.ptr, d, g.ptr, g.ptr + 4 * d, g.ptr + 8 * d, 3 * d,
+        gn = _norm_gradient(ctx, g, acc, Bn * S, d, qk_norm)
+        ctx.check(ctx.lib.fml_attention_bwd(ctx.h, ctypes.byref(desc), out.grad.ptr, d, gn.ptr, gn.ptr + 4 * d, g.ptr + 8 * d, 3 * d,
                                             1 if acc else 0, scratch.ptr))
         ctx.launches += 4
+        if qk_norm is not None:
+            qk_norm.backward(ctx, qkv.value, gn, g, Bn * S, S, H, H, dk, 3 * d, 3 * d, acc)
         _keep = (lse, out)  # the descriptor holds raw pointers into these
-    out.creator = Node([qkv], bw, "attention", 4 * Bn * H * S * S * dk, {"causal": causal, "fused": True})
+    out.creator = Node([qkv] + (qk_norm.inputs if qk_norm is not None else []), bw, "attention", 4 * Bn * H * S * S * dk, {"causal": causal, "fused": True})
     out.attention_weights = None   # never materialised on this path (set FUSE_ATTENTION = False to inspect them)
     return out
 
 
-def attentionCore(qkv: Tensor, n_seq: int, seq_len: int, heads: int, d_head: int, causal: bool, precision: int = -1):
+def _norm_gradient(ctx, g, acc, rows, d, qk_norm):
+    """Where the attention's backward pass leaves the gradients of its queries and keys: in the projection's gradient, or,
+    with a norm between the two, in a buffer of the same form (zeroed when the pass adds)."""
+    if qk_norm is None:
+        return g
+    return ctx.zeros(rows, 3 * d) if acc else ctx.empty(rows, 3 * d)
+
+
+def attentionCore(qkv: Tensor, n_seq: int, seq_len: int, heads: int, d_head: int, causal: bool, precision: int = -1,
+                  qk_norm: Optional[QKNorm] = None):
     """Scaled dot-product attention for all (sequence, head) pairs at once, reading Q, K, V as
     column slices of the fused projection [n_seq*seq_len, 3*heads*d_head] and writing the heads
     side by side: transpose + matMul + scaleMatrix + softmaxMatrix + matMul of
     lib/layertypes/singleHeadAttentionLayer.dart:77-86 and the column concat of
-    lib/transformer/multiHeadAttentionLayer.dart:80, without any of those copies."""
+    lib/transformer/multiHeadAttentionLayer.dart:80, without any of those copies.  With `qk_norm`, queries and keys pass
+    through the norm and rotation first, into a buffer of the same row stride (its third third stays unused)."""
     ctx = qkv.ctx
     Bn, S, H, dk = n_seq, seq_len, heads, d_head
     d = H * dk
     ld = 3 * d
     scale = 1.0 / math.sqrt(dk)
     q, k, v = qkv.value, qkv.value.view(d, ()), qkv.value.view(2 * d, ())
+    if qk_norm is not None:
+        q = ctx.empty(Bn * S, ld)
+        k = q.view(d, ())
+        qk_norm.forward(ctx, qkv.value, q, Bn * S, S, H, H, dk, ld, ld)
     eff_prec = ctx.precision if precision < 0 else precision
     if FUSE_ATTENTION and eff_prec == _lib.PREC_TF32 and dk == 64 and S % 128 == 0:
-        return _attentionFused(qkv, q, k, v, Bn, S, H, dk, causal, scale)
+        return _attentionFused(qkv, q, k, v, Bn, S, H, dk, causal, scale, qk_norm)
     P = ctx.empty(Bn * H * S, S)
     out = Tensor(ctx.empty(Bn * S, d), ctx)
     bat = dict(batch=(H, Bn), precision=precision)
@@ -476,7 +553,8 @@ def attentionCore(qkv: Tensor, n_seq: int, seq_len: int, heads: int, d_head: int
         if not acc:
             pass  # every element of the buffer is written below (dQ, dK, dV cover all 3*d columns)
         beta = 1.0 if acc else 0.0
-        gq, gk, gv = g, g.view(d, ()), g.view(2 * d, ())
+        gn = _norm_gradient(ctx, g, acc, Bn * S, d, qk_norm)
+        gq, gk, gv = gn, gn.view(d, ()), g.view(2 * d, ())
         dO = out.grad
         dP = ctx.empty(Bn * H * S, S)
         # dP = dO_h . V_h^T ; dV_h = P^T . dO_h
@@ -495,7 +573,9 @@ def attentionCore(qkv: Tensor, n_seq: int, seq_len: int, heads: int, d_head: int
         # dQ_h = dS . K_h ; dK_h = dS^T . Q_h
         ctx.gemm(dP, k, gq, S, dk, S, lda=S, ldb=ld, ldc=ld, sA=s_p, sB=s_qkv, sC=s_qkv, beta=beta, **bat)
         ctx.gemm(dP, q, gk, S, dk, S, transA=True, lda=S, ldb=ld, ldc=ld, sA=s_p, sB=s_qkv, sC=s_qkv, beta=beta, **bat)
-    out.creator = Node([qkv], bw, "attention", 4 * Bn * H * S * S * dk, {"causal": causal})
+        if qk_norm is not None:
+            qk_norm.backward(ctx, qkv.value, gn, g, Bn * S, S, H, H, dk, ld, ld, acc)
+    out.creator = Node([qkv] + (qk_norm.inputs if qk_norm is not None else []), bw, "attention", 4 * Bn * H * S * S * dk, {"causal": causal})
     out.attention_weights = P
     return out
 

@@ -477,6 +477,30 @@ int32_t fml_attention_fwd(fml_ctx* ctx, const fml_attention_desc* d);
 int32_t fml_attention_bwd(fml_ctx* ctx, const fml_attention_desc* d, const float* dout, int64_t ld_dout, float* dq,
                           float* dk, float* dv, int64_t ld_dqkv, int32_t accumulate, float* scratch);
 
+/* ---- norm of queries and keys with the position rotation -----------------------------
+ * (Extension: it stands between the projections and the attention of singleHeadAttentionLayer.dart:77-86.)  For every row
+ * and head of q (heads_q heads of d_head columns, row stride ld_q) and of k, in one launch:
+ *   xh = x / sqrt(mean(x^2) + eps),  z = gain * xh,  out = z with the pairs of its first rot_dim columns turned by
+ *   pos * base^(-2 i / rot_dim): pairs (i, i + rot_dim / 2), or (2 i, 2 i + 1) when interleaved != 0.
+ * pos is positions[row] (device, any sign), or row mod seq_len when positions is NULL (seq_len 0: row).  gain_q and gain_k
+ * hold d_head floats, NULL means ones; heads_k may be 0 (k is then ignored) and may differ from heads_q.  d_head is 1 to
+ * 256, rot_dim even and 0 to d_head (0: no rotation).  An output may be its own input (same address and stride) and shares
+ * nothing else with another buffer.
+ * Backward: dq, dk from the forward pass's inputs and the gradients of its outputs, overwritten or added to (accumulate);
+ * dgain_q, dgain_k (either may be NULL) are added to, through `scratch` of FML_QK_NORM_ROPE_PARTS * 2 * d_head floats
+ * (may be NULL when both are). */
+#define FML_QK_NORM_ROPE_PARTS 592
+int32_t fml_qk_norm_rope_fwd(fml_ctx* ctx, const float* q, int64_t ld_q, float* q_out, int64_t ld_q_out, int32_t heads_q,
+                             const float* k, int64_t ld_k, float* k_out, int64_t ld_k_out, int32_t heads_k, int64_t rows,
+                             int32_t d_head, const float* gain_q, const float* gain_k, const int32_t* positions,
+                             int32_t seq_len, int32_t rot_dim, int32_t interleaved, double base, float eps);
+int32_t fml_qk_norm_rope_bwd(fml_ctx* ctx, const float* q, int64_t ld_q, const float* dq_out, int64_t ld_dq_out, float* dq,
+                             int64_t ld_dq, int32_t heads_q, const float* k, int64_t ld_k, const float* dk_out,
+                             int64_t ld_dk_out, float* dk, int64_t ld_dk, int32_t heads_k, int64_t rows, int32_t d_head,
+                             const float* gain_q, const float* gain_k, float* dgain_q, float* dgain_k,
+                             const int32_t* positions, int32_t seq_len, int32_t rot_dim, int32_t interleaved, double base,
+                             float eps, int32_t accumulate, float* scratch);
+
 /* ---- convolution -----------------------------------------------------------------
  * conv2d (tensor.dart:765-833) for every kernel of a Conv2DLayer (lib/layertypes/conv2d.dart:60-75) and every image
  * of a batch in one launch: in [n_img][H][W], w [n_k][kh][kw], bias [n_k] or NULL (addScalarToMatrix,
