@@ -91,6 +91,12 @@ abstract final class FmlTapeDirection {
   static const int FML_TAPE_BACKWARD_NOSEED = 2;
 }
 
+/// `fml_recurrence_form`.
+abstract final class FmlRecurrenceForm {
+  static const int FML_RECURRENCE_GATED = 0;
+  static const int FML_RECURRENCE_LINEAR = 1;
+}
+
 abstract final class FmlLimits {
   static const int FML_XENT_STATIC_MAX_ROWS = 65536;
   static const int FML_QK_NORM_ROPE_PARTS = 592;
@@ -465,6 +471,12 @@ class FmlBindings {
   late final fmlLstmCellBwd = lib.lookupFunction<
       Int32 Function(Pointer<FmlCtx>, Pointer<Float>, Pointer<Float>, Pointer<Float>, Pointer<Float>, Pointer<Float>, Pointer<Float>, Pointer<Float>, Int32, Int64, Int64),
       int Function(Pointer<FmlCtx>, Pointer<Float>, Pointer<Float>, Pointer<Float>, Pointer<Float>, Pointer<Float>, Pointer<Float>, Pointer<Float>, int, int, int)>('fml_lstm_cell_bwd');
+  late final fmlGatedRecurrenceFwd = lib.lookupFunction<
+      Int32 Function(Pointer<FmlCtx>, Int32, Int32, Int32, Int32, Pointer<Float>, Pointer<Float>, Int64, Int64, Pointer<Float>, Pointer<Int32>, Pointer<Float>, Int64, Int64, Pointer<Float>),
+      int Function(Pointer<FmlCtx>, int, int, int, int, Pointer<Float>, Pointer<Float>, int, int, Pointer<Float>, Pointer<Int32>, Pointer<Float>, int, int, Pointer<Float>)>('fml_gated_recurrence_fwd');
+  late final fmlGatedRecurrenceBwd = lib.lookupFunction<
+      Int32 Function(Pointer<FmlCtx>, Int32, Int32, Int32, Int32, Pointer<Float>, Pointer<Float>, Int64, Int64, Pointer<Float>, Pointer<Int32>, Pointer<Float>, Pointer<Float>, Int64, Int64, Pointer<Float>, Pointer<Float>, Pointer<Float>, Pointer<Float>, Int32),
+      int Function(Pointer<FmlCtx>, int, int, int, int, Pointer<Float>, Pointer<Float>, int, int, Pointer<Float>, Pointer<Int32>, Pointer<Float>, Pointer<Float>, int, int, Pointer<Float>, Pointer<Float>, Pointer<Float>, Pointer<Float>, int)>('fml_gated_recurrence_bwd');
   late final fmlDpUniqueId = lib.lookupFunction<
       Int32 Function(Pointer<Uint8>),
       int Function(Pointer<Uint8>)>('fml_dp_unique_id');

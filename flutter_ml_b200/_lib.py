@@ -20,6 +20,7 @@ ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_TANH, ACT_GELU = 0, 1, 2, 3, 4
 ACT_BY_NAME = {None: ACT_NONE, "none": ACT_NONE, "relu": ACT_RELU, "sigmoid": ACT_SIGMOID, "tanh": ACT_TANH,
                "gelu": ACT_GELU}
 
+RECURRENCE_BY_NAME = {"gated": 0, "linear": 1}
 QK_NORM_ROPE_PARTS = 592   # partial sums of the gain gradients, one a CTA (FML_QK_NORM_ROPE_PARTS)
 
 i32, i64, f32 = C.c_int32, C.c_int64, C.c_float
@@ -154,6 +155,8 @@ PROTOTYPES = {
     "fml_lstm_bwd": [fp, C.POINTER(LstmDesc), fp, fp, fp, fp, fp],
     "fml_lstm_cell_fwd": [fp, fp, fp, fp, fp, fp, i64, i64],
     "fml_lstm_cell_bwd": [fp, fp, fp, fp, fp, fp, fp, fp, i32, i64, i64],
+    "fml_gated_recurrence_fwd": [fp, i32, i32, i32, i32, fp, fp, i64, i64, fp, fp, fp, i64, i64, fp],
+    "fml_gated_recurrence_bwd": [fp, i32, i32, i32, i32, fp, fp, i64, i64, fp, fp, fp, fp, i64, i64, fp, fp, fp, fp, i32],
     "fml_dp_unique_id": [C.c_char_p],
     "fml_dp_init": [fp, C.c_char_p, i32, i32],
     "fml_dp_set_timeout": [fp, i32],

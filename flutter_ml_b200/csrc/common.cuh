@@ -103,7 +103,8 @@ int32_t fml_ensure_workspace_keep(fml_ctx* ctx, size_t bytes);
 // Second word of the context's status block: set (first writer wins) by a kernel that met a token id or a class label
 // outside its range.  The kernel skips the access, so a bad index is a reported error, never an illegal address.
 #define FML_STATUS_BAD_INDEX_WORD 1
-enum { FML_BAD_INDEX_EMBEDDING_FWD = 201, FML_BAD_INDEX_EMBEDDING_BWD = 202, FML_BAD_INDEX_LABEL = 203 };
+enum { FML_BAD_INDEX_EMBEDDING_FWD = 201, FML_BAD_INDEX_EMBEDDING_BWD = 202, FML_BAD_INDEX_LABEL = 203,
+       FML_BAD_INDEX_LENGTH = 204 };
 __device__ __forceinline__ void fml_flag_bad_index(int* status, int code) {
   if (status) atomicCAS(status + FML_STATUS_BAD_INDEX_WORD, 0, code);
 }

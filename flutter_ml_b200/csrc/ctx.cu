@@ -204,8 +204,10 @@ int32_t fml_device_status(fml_ctx* ctx, int32_t* code) {
   if (v[1] != 0) {
     cudaMemsetAsync(ctx->d_status + FML_STATUS_BAD_INDEX_WORD, 0, sizeof(int), ctx->stream);
     return fml_fail(ctx, FML_ERR_INVALID,
-                    std::string(v[1] == FML_BAD_INDEX_LABEL ? "a class label was outside [0, cols)" : "a token id was outside [0, vocab)") +
-                        "; the access was skipped (code " + std::to_string(v[1]) + ")");
+                    std::string(v[1] == FML_BAD_INDEX_LABEL    ? "a class label was outside [0, cols)"
+                                : v[1] == FML_BAD_INDEX_LENGTH ? "a sequence length was outside [0, seq_len] and taken as the nearest of the two"
+                                                               : "a token id was outside [0, vocab)") +
+                        (v[1] == FML_BAD_INDEX_LENGTH ? " (code " : "; the access was skipped (code ") + std::to_string(v[1]) + ")");
   }
   return FML_OK;
 }

@@ -204,6 +204,41 @@ class LSTMLayer(Layer):
         return out
 
 
+class GatedRecurrentLayer(Layer):
+    """Recurrent layer whose gates read the input alone (extension beside LSTMLayer): one product x.W + b gives gates and
+    candidates for all steps, the gated linear recurrence joins them, so there is no product in the loop over time.
+
+    Input: a batch of sequences flattened into rows [n_seq * seq_len x I] (one sequence when seq_len is None); output: every
+    state [n_seq * seq_len x H], or with returnSequences=False the last of each sequence [n_seq x H].  `call(x)` takes full
+    sequences; `forward(x, lens=..., h0=...)` ragged ones and a state to start from.  W [I x 2 H] = [gates | candidates],
+    He-normal like the dense layers; gate biases 1 (the state is kept by default), candidate biases 0, unless given."""
+    name = "gated_recurrent"
+
+    def __init__(self, hiddenSize: int, seq_len: Optional[int] = None, returnSequences: bool = True, seed: int = 0, weights=None, bias=None,
+                 precision: int = -1):
+        super().__init__()
+        self.hiddenSize, self.seq_len, self.returnSequences = hiddenSize, seq_len, returnSequences
+        self.seed, self._w0, self._b0, self.precision = seed, weights, bias, precision
+        self.weights: Optional[Tensor] = None
+        self.biases: Optional[Tensor] = None
+
+    @property
+    def parameters(self):
+        return [self.weights, self.biases]
+
+    def build(self, x: Tensor):
+        H, I = self.hiddenSize, x.shape[1]
+        w = self._w0 if self._w0 is not None else synth.normal(self.seed, 0, (I, 2 * H), math.sqrt(2.0 / I))
+        b = self._b0 if self._b0 is not None else np.concatenate([np.ones(H), np.zeros(H)]).astype(np.float32)
+        self.weights, self.biases = Tensor(w, x.ctx), Tensor(b, x.ctx)
+        super().build(x)
+
+    def forward(self, x: Tensor, lens=None, h0: Optional[Tensor] = None) -> Tensor:
+        S = self.seq_len or x.shape[0]
+        z = T.denseMatrix(x, self.weights, self.biases, None, self.precision)
+        return T.gatedRecurrence(z, x.shape[0] // S, S, "gated", h0, lens, "all" if self.returnSequences else "last")
+
+
 class MultiTierLSTMLayer(Layer):
     """MultiTierLSTMLayer (lib/layertypes/multilstm.dart:14-208): a stack of LSTM tiers on different clocks.
 

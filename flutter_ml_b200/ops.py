@@ -175,6 +175,25 @@ class DenseFwdBwdHost:
         return self.h_out
 
 
+def gated_recurrence_forward(ctx, f, x, h, n_seq, seq_len, dim, form="gated", h0=None, lens=None, h_last=None, strides_in=None, strides_h=None):
+    """h_t = a_t h_{t-1} + (1 - a_t) x_t with a = sigmoid(f) (form "gated"), or h_t = f_t h_{t-1} + x_t ("linear"), along every
+    sequence (`fml_gated_recurrence_fwd`).  strides_in (f and x) and strides_h are (sequence, step) strides in elements,
+    sequence-major without gaps by default; lens: int32 lengths on the device."""
+    dense = (seq_len * dim, dim)
+    si, sh = strides_in or dense, strides_h or dense
+    ctx.call("fml_gated_recurrence_fwd", _lib.RECURRENCE_BY_NAME[form], n_seq, seq_len, dim, f, x, si[0], si[1], h0, lens, h, sh[0], sh[1], h_last)
+
+
+def gated_recurrence_backward(ctx, f, x, h, dy, df, dx, n_seq, seq_len, dim, form="gated", h0=None, lens=None, dh_last=None, dh0=None,
+                              strides_in=None, strides_h=None, accumulate=False):
+    """Gradients of `gated_recurrence_forward` from its inputs and its h (`fml_gated_recurrence_bwd`); dy may be None (zero),
+    df and dx lie at the strides of f and x, dy at those of h."""
+    dense = (seq_len * dim, dim)
+    si, sh = strides_in or dense, strides_h or dense
+    ctx.call("fml_gated_recurrence_bwd", _lib.RECURRENCE_BY_NAME[form], n_seq, seq_len, dim, f, x, si[0], si[1], h0, lens, h, dy, sh[0], sh[1],
+             dh_last, df, dx, dh0, 1 if accumulate else 0)
+
+
 def qk_norm_rope_scratch(d_head: int) -> int:
     """Floats of the scratch buffer that the gain gradients of `qk_norm_rope_backward` go through."""
     return _lib.QK_NORM_ROPE_PARTS * 2 * d_head

@@ -580,6 +580,45 @@ def attentionCore(qkv: Tensor, n_seq: int, seq_len: int, heads: int, d_head: int
     return out
 
 
+def gatedRecurrence(z: Tensor, n_seq: int, seq_len: int, form: str = "gated", h0: Optional[Tensor] = None,
+                    lens: Optional[DeviceArray] = None, output: str = "all") -> Tensor:
+    """The gated linear recurrence along n_seq sequences of seq_len rows each (sequence-major, as everywhere in this module).
+    z [n_seq * seq_len x 2 H] is one projection: gates f in its first H columns, inputs x behind them (form "gated":
+    h_t = a_t h_{t-1} + (1 - a_t) x_t, a = sigmoid(f); "linear": h_t = f_t h_{t-1} + x_t).  h0: [n_seq x H] or None; lens: int32
+    lengths on the device or None.  output "all": every state [n_seq * seq_len x H], rows behind a sequence's end zero;
+    "last": the state after each sequence's last step [n_seq x H].  Extension beside lib/layertypes/lstmLayer.dart:112-150."""
+    ctx = z.ctx
+    R, W = z.shape
+    if W % 2 or R != n_seq * seq_len:
+        raise ValueError(f"gatedRecurrence: {n_seq} x {seq_len} rows of gates and inputs expected, got {z.shape}")
+    if output not in ("all", "last"):
+        raise ValueError("gatedRecurrence: output is 'all' or 'last'")
+    H = W // 2
+    if h0 is not None and h0.value.size != n_seq * H:
+        raise ValueError("gatedRecurrence: h0 must be [n_seq x H]")
+    if lens is not None and (lens.dtype != np.int32 or lens.size != n_seq):
+        raise ValueError("gatedRecurrence: lens must be int32, one for each sequence")
+    last = output == "last"
+    h = ctx.zeros(R, H) if lens is not None else ctx.empty(R, H)
+    end = ctx.empty(n_seq, H) if last else None
+    size = dict(n_seq=n_seq, seq_len=seq_len, dim=H, form=form, lens=lens, strides_in=(seq_len * W, W))
+    h0v = h0.value if h0 is not None else None
+    ops.gated_recurrence_forward(ctx, z.value, z.value.view(H, ()), h, h0=h0v, h_last=end, **size)
+    out = Tensor(end if last else h, ctx)
+
+    def bw():
+        g, acc = z._grad_target()
+        g0, acc0 = h0._grad_target() if h0 is not None else (None, acc)
+        if acc != acc0:                       # one of the two is new: both are added to
+            ctx.zero(g0 if acc else g)
+        elif not acc and lens is not None:    # rows behind the ends are not written
+            ctx.zero(g)
+        ops.gated_recurrence_backward(ctx, z.value, z.value.view(H, ()), h, None if last else out.grad, g, g.view(H, ()), h0=h0v,
+                                      dh_last=out.grad if last else None, dh0=g0, accumulate=acc or acc0, **size)
+    out.creator = Node([z] + ([h0] if h0 is not None else []), bw, "gated_recurrence", 10 * R * H, {"form": form})
+    return out
+
+
 def conv2dBatch(x: Tensor, kernels: Tensor, biases: Optional[Tensor], kh: int, kw: int, padding: str = "valid") -> Tensor:
     """conv2d (tensor.dart:765-833) of every image in x [n_img, H, W] with every kernel in `kernels`
     [n_k, kh*kw] (x may also be one matrix [H, W]), plus addScalarToMatrix of `biases` [n_k] (tensor.dart:711-737): Conv2DLayer.forward

@@ -80,7 +80,9 @@ int32_t fml_sync(fml_ctx* ctx);
 /* What kernels could not do, read back once (reading synchronises, then clears):
  *   - a bounded device-side wait that expired instead of hanging: returns FML_ERR_TIMEOUT, *code = the role that gave up;
  *   - a token id or class label outside its range (201 embedding forward, 202 embedding backward, 203 cross-entropy
- *     label): returns FML_ERR_INVALID, *code = which.  The kernel skipped the access, so memory is intact.
+ *     label): returns FML_ERR_INVALID, *code = which.  The kernel skipped the access, so memory is intact;
+ *   - a sequence length of the gated recurrence outside [0, seq_len]: FML_ERR_INVALID, *code = 204; the nearest of the two
+ *     was used.
  * 0 / FML_OK means neither happened. */
 int32_t fml_device_status(fml_ctx* ctx, int32_t* code);
 /* Failure-path self test: one CTA waits (with the bounded wait all pipeline roles use) on a barrier that nothing
@@ -554,6 +556,32 @@ int32_t fml_lstm_bwd(fml_ctx* ctx, const fml_lstm_desc* d, const float* dh_last,
 int32_t fml_lstm_cell_fwd(fml_ctx* ctx, const float* pre, const float* c_prev, float* gates, float* c, float* h, int64_t B, int64_t H);
 int32_t fml_lstm_cell_bwd(fml_ctx* ctx, const float* gates, const float* c_prev, const float* c, const float* dh, const float* dc,
                           float* dpre, float* dc_prev, int32_t accumulate_dc_prev, int64_t B, int64_t H);
+
+/* ---- gated linear recurrence ---------------------------------------------------
+ * (Extension beside the LSTM: gates that do not read the state, so the steps can be joined in any grouping.)  For every
+ * sequence s, channel c and step t < lens[s] (lens NULL: seq_len), from h0 [n_seq][dim] (NULL: zero):
+ *   FML_RECURRENCE_GATED   a = sigmoid(f),  h_t = a h_{t-1} + (1 - a) x_t
+ *   FML_RECURRENCE_LINEAR  a = f,           h_t = a h_{t-1} + x_t
+ * Element (s, t, c) of f and x lies at s * seq_stride_in + t * step_stride_in + c (elements; both arrays share the strides,
+ * so they may be the halves of one fused projection), of h at the strides of h: sequence-major, time-major and sliced
+ * layouts alike.  h_last [n_seq][dim] (or NULL) receives the state after each sequence's last step and may be h0 itself.
+ * Rows of h behind a sequence's end are left as they were.  A length outside [0, seq_len] (device memory) is reported by
+ * fml_device_status and taken as the nearest of the two.  One step at a time is the same call with seq_len = 1.
+ * LINEAR: the decays of up to 512 neighbouring steps are multiplied in float32; where such a product leaves float32's
+ * range while the states do not, the result is the one with the product at infinity or zero.
+ * Backward, from the forward call's inputs and its h: dy (strides of h; NULL: zero) and dh_last (NULL: zero) are the
+ * gradients of h and h_last; df and dx (strides of f and x) and dh0 (NULL: not wanted) are overwritten, or added to when
+ * accumulate != 0; rows behind a sequence's end are left as they were.  dh0 may be dh_last itself when nothing is added.
+ * No output may share memory with another buffer in any other way. */
+typedef enum { FML_RECURRENCE_GATED = 0, FML_RECURRENCE_LINEAR = 1 } fml_recurrence_form;
+int32_t fml_gated_recurrence_fwd(fml_ctx* ctx, int32_t form, int32_t n_seq, int32_t seq_len, int32_t dim, const float* f,
+                                 const float* x, int64_t seq_stride_in, int64_t step_stride_in, const float* h0,
+                                 const int32_t* lens, float* h, int64_t seq_stride_h, int64_t step_stride_h, float* h_last);
+int32_t fml_gated_recurrence_bwd(fml_ctx* ctx, int32_t form, int32_t n_seq, int32_t seq_len, int32_t dim, const float* f,
+                                 const float* x, int64_t seq_stride_in, int64_t step_stride_in, const float* h0,
+                                 const int32_t* lens, const float* h, const float* dy, int64_t seq_stride_h,
+                                 int64_t step_stride_h, const float* dh_last, float* df, float* dx, float* dh0,
+                                 int32_t accumulate);
 
 /* ---- data parallel (one process per GPU) -------------------------------------
  * The reference has no multi-device code.  Rank 0 creates an id, the host
