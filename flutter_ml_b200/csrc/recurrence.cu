@@ -24,10 +24,11 @@
 #include <cstdlib>
 
 #include "common.cuh"
+#include "tc_ptx.cuh"
 
 namespace {
 
-constexpr int WARPS = 8, THREADS = 32 * WARPS;
+constexpr int THREADS = 256;
 constexpr int MAX_CLUSTER = 8;
 
 struct Params {
@@ -36,36 +37,38 @@ struct Params {
   float *out, *last;            // forward: h, h_last
   float *df, *dx, *dh0;         // backward
   long long ss_in, ts_in, ss_h, ts_h;
-  int n_seq, seq_len, dim, ctiles, cluster, accumulate;
+  int n_seq, seq_len, dim, ctiles, accumulate;
+  int cluster;                  // CTAs that share the steps of a sequence
   int* status;
 };
 
-// a and s = 1 - a without the difference: whichever is small comes from the exponential itself
+// a = 1 / (1 + e), s = 1 - a = e a with e = exp(-f): neither is a difference, both keep their relative precision (4 u of the
+// exponential, 1.2 |f| u of its argument in base 2, 2 u of the reciprocal, u = 2^-24).  Gates below -80 count as -80: e stays
+// finite, a is 2e-35.  The hardware's exponential and reciprocal, six instructions: with expf and a division the forward
+// scan issued 40 instructions an element and was bound by them.
 template <bool GATED>
 __device__ __forceinline__ void gate(float f, float& a, float& s) {
   if (GATED) {
-    const float e = expf(-fabsf(f)), big = __fdividef(1.f, 1.f + e), small = e * big;
-    a = f >= 0.f ? big : small;
-    s = f >= 0.f ? small : big;
+    float g, r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(g) : "f"(f), "f"(-80.f));
+    const float e = fml_exp2_ftz(-1.4426950408889634f * g);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    a = r;
+    s = e * r;
   } else {
     a = f;
     s = 1.f;
   }
 }
 
-// "state <- A state + B"; a zero state stays clear of a product of decays that has overflowed
-__device__ __forceinline__ float through(float A, float B, float state) { return state == 0.f ? B : fmaf(A, state, B); }
+// "state <- A state + B".  LINEAR decays may be above one: a zero state stays clear of a product of them that has overflowed
+template <bool GATED>
+__device__ __forceinline__ float through(float A, float B, float state) { return !GATED && state == 0.f ? B : fmaf(A, state, B); }
 
-__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void store_remote(const float2* here, uint32_t rank, float2 v) {
-  const uint32_t at = (uint32_t)__cvta_generic_to_shared(here);
+__device__ __forceinline__ void store_remote(const float* here, uint32_t rank, float v) {
   uint32_t there;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
-  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(there), "f"(v.x), "f"(v.y) : "memory");
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(fml_tc::smem_u32(here)), "r"(rank));
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(v) : "memory");
 }
 
 __device__ __forceinline__ int length_of(const Params& p, int seq) {
@@ -75,121 +78,250 @@ __device__ __forceinline__ int length_of(const Params& p, int seq) {
   return min(max(n, 0), p.seq_len);
 }
 
-template <int CW, int SEG, bool GATED, bool BWD>
-__global__ void __launch_bounds__(THREADS) scan_kernel(const Params p) {
-  constexpr int SUBS = 32 / CW;                       // lanes that share a channel
+template <int VEC>
+__device__ __forceinline__ void load_row(float* dst, const float* src) {
+  if (VEC == 4) *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(src);
+  else if (VEC == 2) *reinterpret_cast<float2*>(dst) = *reinterpret_cast<const float2*>(src);
+  else *dst = *src;
+}
+template <int VEC>
+__device__ __forceinline__ void store_row(float* dst, const float* src) {
+  if (VEC == 4) *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(src);
+  else if (VEC == 2) *reinterpret_cast<float2*>(dst) = *reinterpret_cast<const float2*>(src);
+  else *dst = *src;
+}
+
+// What a lane has read of its segment, SEG steps of VEC channels, in scan direction.
+template <int VEC, int SEG, bool BWD>
+struct Raw {
+  float f[SEG][VEC], x[SEG][VEC];
+  float dy[BWD ? SEG : 1][VEC], hp[BWD ? SEG : 1][VEC];
+};
+
+// Steps behind the end become a gate of one and an input of zero: the state passes through them.
+template <int VEC, int SEG, bool GATED, bool BWD>
+__device__ __forceinline__ void load_segment(const Params& p, Raw<VEC, SEG, BWD>& r, const float* f, const float* x, const float* h,
+                                             const float* dy, const float* first, int p0, int len, bool on) {
+  const int t0 = BWD ? len - 1 - p0 : p0;             // the first step's place; backward they descend
+  const long long di = BWD ? -p.ts_in : p.ts_in;
+  f += t0 * p.ts_in;
+  x += t0 * p.ts_in;
+  if (BWD) {
+    h += (t0 - 1) * p.ts_h;                           // the state before the step
+    dy += t0 * p.ts_h;
+  }
+  // wholly inside (backward: without step 0, whose state before is h0): no tests
+  if (on && p0 + SEG + (BWD ? 1 : 0) <= len && (!BWD || p.dy)) {
+#pragma unroll
+    for (int i = 0; i < SEG; i++) {
+      load_row<VEC>(r.f[i], f + i * di);
+      if (GATED || !BWD) load_row<VEC>(r.x[i], x + i * di);
+      if (BWD) {
+        load_row<VEC>(r.hp[i], h - i * p.ts_h);
+        load_row<VEC>(r.dy[i], dy - i * p.ts_h);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < SEG; i++) {
+    const bool there = on && p0 + i < len;
+#pragma unroll
+    for (int v = 0; v < VEC; v++) {
+      r.f[i][v] = GATED ? INFINITY : 1.f;
+      r.x[i][v] = 0.f;
+      if (BWD) {
+        r.dy[i][v] = 0.f;
+        r.hp[i][v] = first[v];
+      }
+    }
+    if (!there) continue;
+    load_row<VEC>(r.f[i], f + i * di);
+    if (GATED || !BWD) load_row<VEC>(r.x[i], x + i * di);
+    if (BWD) {
+      if (p.dy) load_row<VEC>(r.dy[i], dy - i * p.ts_h);
+      if (p0 + i < len - 1) load_row<VEC>(r.hp[i], h - i * p.ts_h);
+    }
+  }
+}
+
+template <int WARPS, int LANES, int VEC, int SEG, bool GATED, bool BWD, bool AHEAD, bool TEAM>
+__global__ void __launch_bounds__(32 * WARPS) scan_kernel(const Params p) {
+  constexpr int SUBS = 32 / LANES;                    // segments of a warp that share their channels
+  constexpr int CW = LANES * VEC;                     // channels of a CTA
   constexpr int TILE = WARPS * SUBS * SEG;            // steps of a CTA's round
-  __shared__ float2 wtot[2][WARPS][CW];               // the warps' pairs; two sets, so one barrier a round is enough
-  __shared__ float2 ctot[2][MAX_CLUSTER][CW];         // the CTAs' pairs, written by their owners into every CTA
+  __shared__ __align__(16) float wtot[2][WARPS][2][CW];   // the warps' pairs; two sets, so one barrier a round is enough
+  __shared__ __align__(16) float ctot[TEAM ? 2 : 1][TEAM ? MAX_CLUSTER : 1][2][CW];   // the CTAs' pairs, written by their owners into every CTA
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int ch = lane % CW, sub = lane / CW;
-  const int cs = p.cluster;
-  const int rank = cs > 1 ? (int)cluster_rank() : 0;
+  const int ch = (lane % LANES) * VEC, sub = lane / LANES;
+  const int cs = TEAM ? p.cluster : 1, rank = TEAM ? (int)fml_tc::cluster_ctarank() : 0;
   const int unit = blockIdx.x / cs;
   const int seq = unit / p.ctiles, c = (unit - seq * p.ctiles) * CW + ch;
   const bool on = c < p.dim;
   const int len = length_of(p, seq);
   const float* f = p.f + seq * p.ss_in + c;
   const float* x = p.x + seq * p.ss_in + c;
+  const float* h = p.h + seq * p.ss_h + c;
+  const float* dy = p.dy + seq * p.ss_h + c;
   const long long edge = (long long)seq * p.dim + c;  // of h0, h_last and their gradients
-  float state = 0.f;
-  const float first = on && p.h0 ? p.h0[edge] : 0.f;  // h before step 0
-  if (!BWD) state = first;
-  else if (on && p.dh_last) state = p.dh_last[edge];
-  if (cs > 1) cluster_sync();                         // every CTA is there before the first remote store
-  int buf = 0;
-  for (int base = 0; base < len; base += TILE * cs, buf ^= 1) {
-    const int p0 = base + ((rank * WARPS + warp) * SUBS + sub) * SEG;   // first step of the segment, counted in scan direction
-    float a[SEG], s[SEG], xv[SEG], b[SEG], hp[SEG];   // what a form or direction does not use, the compiler drops
+  float state[VEC], first[VEC];                       // first: h before step 0
 #pragma unroll
-    for (int i = 0; i < SEG; i++) {
-      const int q = p0 + i;
-      const bool there = on && q < len;
-      const int t = BWD ? len - 1 - q : q;
-      a[i] = there ? f[t * p.ts_in] : 0.f;
-      xv[i] = there && (GATED || !BWD) ? x[t * p.ts_in] : 0.f;
-      if (BWD) {
-        b[i] = there && p.dy ? p.dy[seq * p.ss_h + t * p.ts_h + c] : 0.f;
-        hp[i] = there && t > 0 ? p.h[seq * p.ss_h + (t - 1) * p.ts_h + c] : first;
+  for (int v = 0; v < VEC; v++) {
+    first[v] = on && p.h0 ? p.h0[edge + v] : 0.f;
+    state[v] = !BWD ? first[v] : on && p.dh_last ? p.dh_last[edge + v] : 0.f;
+  }
+  Raw<VEC, SEG, BWD> raw;
+  if (TEAM) fml_tc::cluster_sync_all();               // every CTA is there before the first remote store
+  int p0 = ((rank * WARPS + warp) * SUBS + sub) * SEG;   // first step of the segment, counted in scan direction
+  if (AHEAD) load_segment<VEC, SEG, GATED, BWD>(p, raw, f, x, h, dy, first, p0, len, on);
+  for (int base = 0, buf = 0; base < len; base += TILE * cs, p0 += TILE * cs, buf ^= 1) {
+    if (!AHEAD) load_segment<VEC, SEG, GATED, BWD>(p, raw, f, x, h, dy, first, p0, len, on);
+    // forward: decay and input; backward: decay, incoming gradient, and what G is multiplied by for dx and df
+    float a[SEG][VEC], b[SEG][VEC], s[BWD && GATED ? SEG : 1][VEC], w[BWD ? SEG : 1][VEC];
+    float A[VEC], B[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; v++) {
+      A[v] = 1.f;
+      B[v] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < SEG; i++)
+#pragma unroll
+      for (int v = 0; v < VEC; v++) {
+        float s1;
+        gate<GATED>(raw.f[i][v], a[i][v], s1);
+        if (!BWD) {
+          b[i][v] = GATED ? s1 * raw.x[i][v] : raw.x[i][v];
+          B[v] = fmaf(a[i][v], B[v], b[i][v]);
+        } else {
+          b[i][v] = raw.dy[i][v];
+          B[v] = a[i][v] * (B[v] + b[i][v]);
+          if (GATED) s[i][v] = s1;
+          w[i][v] = GATED ? (raw.hp[i][v] - raw.x[i][v]) * (a[i][v] * s1) : raw.hp[i][v];
+        }
+        A[v] *= a[i][v];
       }
-    }
-    float A = 1.f, B = 0.f;
-#pragma unroll
-    for (int i = 0; i < SEG; i++) {
-      gate<GATED>(a[i], a[i], s[i]);
-      if (!(p0 + i < len)) a[i] = 1.f;                // behind the end: the state passes through (b and xv are 0)
-      if (!BWD) b[i] = s[i] * xv[i];
-      A *= a[i];
-      B = BWD ? a[i] * (B + b[i]) : fmaf(a[i], B, b[i]);
-    }
-    // over the lanes of a channel: the pair of everything before this lane in the warp, and the warp's
-    float Ae = 1.f, Be = 0.f;
+    if (AHEAD) load_segment<VEC, SEG, GATED, BWD>(p, raw, f, x, h, dy, first, p0 + TILE * cs, len, on);
+    // over the segments of the warp: the pair of everything before this one, and the warp's
+    float Ae[VEC], Be[VEC];
     if (SUBS > 1) {
 #pragma unroll
-      for (int o = 1; o < SUBS; o <<= 1) {
-        const float Ap = __shfl_up_sync(0xffffffffu, A, o * CW), Bp = __shfl_up_sync(0xffffffffu, B, o * CW);
-        if (sub >= o) {
-          B = through(A, B, Bp);
-          A *= Ap;
+      for (int o = 1; o < SUBS; o <<= 1)
+#pragma unroll
+        for (int v = 0; v < VEC; v++) {
+          const float Ap = __shfl_up_sync(0xffffffffu, A[v], o * LANES), Bp = __shfl_up_sync(0xffffffffu, B[v], o * LANES);
+          if (sub >= o) {
+            B[v] = through<GATED>(A[v], B[v], Bp);
+            A[v] *= Ap;
+          }
         }
+#pragma unroll
+      for (int v = 0; v < VEC; v++) {
+        Ae[v] = __shfl_up_sync(0xffffffffu, A[v], LANES);
+        Be[v] = __shfl_up_sync(0xffffffffu, B[v], LANES);
       }
-      Ae = __shfl_up_sync(0xffffffffu, A, CW);
-      Be = __shfl_up_sync(0xffffffffu, B, CW);
     }
-    if (sub == SUBS - 1) wtot[buf][warp][ch] = make_float2(A, B);
+    if (sub == SUBS - 1) {
+      store_row<VEC>(&wtot[buf][warp][0][ch], A);
+      store_row<VEC>(&wtot[buf][warp][1][ch], B);
+    }
     __syncthreads();
-    if (cs > 1) {
-      float At = 1.f, Bt = 0.f;
+    float run[VEC];                                   // the state before the lane's steps; `state`: after the round
+    if (TEAM) {
+      // the CTA's pair into every CTA of the cluster; two sets of places, so one cluster barrier a round is enough
+      for (int i = threadIdx.x; i < cs * CW; i += 32 * WARPS) {
+        const int r = i / CW, k = i - r * CW;
+        float At = 1.f, Bt = 0.f;
 #pragma unroll
-      for (int w = 0; w < WARPS; w++) {
-        const float2 v = wtot[buf][w][ch];
-        Bt = through(v.x, v.y, Bt);
-        At *= v.x;
-      }
-      for (int r = warp; r < cs; r += WARPS)
-        if (sub == 0) store_remote(&ctot[buf][rank][ch], r, make_float2(At, Bt));
-      __syncwarp();
-      cluster_sync();
-    }
-    float mine = state;                               // the state before this CTA's steps
-    if (cs > 1) {
-      for (int r = 0; r < cs; r++) {
-        const float2 v = ctot[buf][r][ch];
-        if (r == rank) mine = state;
-        state = through(v.x, v.y, state);
-      }
-    }
-    float run = mine;
-#pragma unroll
-    for (int w = 0; w < WARPS; w++) {
-      if (w == warp) run = mine;
-      const float2 v = wtot[buf][w][ch];
-      mine = through(v.x, v.y, mine);
-    }
-    if (cs == 1) state = mine;
-    if (SUBS > 1 && sub > 0) run = through(Ae, Be, run);
-#pragma unroll
-    for (int i = 0; i < SEG; i++) {
-      const int q = p0 + i;
-      const bool there = on && q < len;
-      if (!BWD) {
-        run = fmaf(a[i], run, b[i]);
-        if (there) p.out[seq * p.ss_h + q * p.ts_h + c] = run;
-      } else {
-        const float G = b[i] + run;
-        run = a[i] * G;
-        const float gx = GATED ? s[i] * G : G;
-        const float gf = GATED ? G * (hp[i] - xv[i]) * (a[i] * s[i]) : G * hp[i];
-        if (there) {
-          const long long at = seq * p.ss_in + (len - 1 - q) * p.ts_in + c;
-          p.dx[at] = p.accumulate ? __fadd_rn(p.dx[at], gx) : gx;
-          p.df[at] = p.accumulate ? __fadd_rn(p.df[at], gf) : gf;
+        for (int q = 0; q < WARPS; q++) {
+          const float Aq = wtot[buf][q][0][k];
+          Bt = through<GATED>(Aq, wtot[buf][q][1][k], Bt);
+          At *= Aq;
         }
+        store_remote(&ctot[buf][rank][0][k], r, At);
+        store_remote(&ctot[buf][rank][1][k], r, Bt);
+      }
+      __syncwarp();
+      fml_tc::cluster_sync_all();
+      for (int r = 0; r < cs; r++) {
+        float Ar[VEC], Br[VEC];
+        load_row<VEC>(Ar, &ctot[buf][r][0][ch]);
+        load_row<VEC>(Br, &ctot[buf][r][1][ch]);
+#pragma unroll
+        for (int v = 0; v < VEC; v++) {
+          if (r == rank) run[v] = state[v];
+          state[v] = through<GATED>(Ar[v], Br[v], state[v]);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < WARPS - 1; q++)
+        if (q < warp) {
+          float Aq[VEC], Bq[VEC];
+          load_row<VEC>(Aq, &wtot[buf][q][0][ch]);
+          load_row<VEC>(Bq, &wtot[buf][q][1][ch]);
+#pragma unroll
+          for (int v = 0; v < VEC; v++) run[v] = through<GATED>(Aq[v], Bq[v], run[v]);
+        }
+    } else {
+#pragma unroll
+      for (int q = 0; q < WARPS; q++) {
+        float Aq[VEC], Bq[VEC];
+        load_row<VEC>(Aq, &wtot[buf][q][0][ch]);
+        load_row<VEC>(Bq, &wtot[buf][q][1][ch]);
+#pragma unroll
+        for (int v = 0; v < VEC; v++) {
+          if (q == warp) run[v] = state[v];
+          state[v] = through<GATED>(Aq[v], Bq[v], state[v]);
+        }
+      }
+    }
+    if (SUBS > 1 && sub > 0) {
+#pragma unroll
+      for (int v = 0; v < VEC; v++) run[v] = through<GATED>(Ae[v], Be[v], run[v]);
+    }
+#pragma unroll
+    for (int i = 0; i < SEG; i++)
+#pragma unroll
+      for (int v = 0; v < VEC; v++) {
+        if (!BWD) {
+          run[v] = b[i][v] = fmaf(a[i][v], run[v], b[i][v]);
+        } else {
+          const float G = b[i][v] + run[v];
+          run[v] = a[i][v] * G;
+          b[i][v] = GATED ? s[i][v] * G : G;          // dx
+          w[i][v] *= G;                               // df
+        }
+      }
+    if (!on || p0 >= len) continue;
+    const int there = len - p0;                       // steps of the segment that exist, or more
+    if (!BWD) {
+      float* to = p.out + seq * p.ss_h + p0 * p.ts_h + c;
+#pragma unroll
+      for (int i = 0; i < SEG; i++)
+        if (i < there) store_row<VEC>(to + i * p.ts_h, b[i]);
+    } else {
+      const long long at = seq * p.ss_in + (len - 1 - p0) * p.ts_in + c;
+      float *tx = p.dx + at, *tf = p.df + at;
+#pragma unroll
+      for (int i = 0; i < SEG; i++) {
+        if (i >= there) break;
+        if (p.accumulate) {
+#pragma unroll
+          for (int v = 0; v < VEC; v++) {
+            b[i][v] = __fadd_rn(tx[v - i * p.ts_in], b[i][v]);
+            w[i][v] = __fadd_rn(tf[v - i * p.ts_in], w[i][v]);
+          }
+        }
+        store_row<VEC>(tx - i * p.ts_in, b[i]);
+        store_row<VEC>(tf - i * p.ts_in, w[i]);
       }
     }
   }
   float* last = BWD ? p.dh0 : p.last;
-  if (last && on && rank == 0 && warp == 0 && sub == 0) last[edge] = BWD && p.accumulate ? __fadd_rn(last[edge], state) : state;
+  if (last && on && rank == 0 && warp == 0 && sub == 0) {
+#pragma unroll
+    for (int v = 0; v < VEC; v++) last[edge + v] = BWD && p.accumulate ? __fadd_rn(last[edge + v], state[v]) : state[v];
+  }
 }
 
 // One thread a channel: single tokens and very short sequences.
@@ -273,21 +405,47 @@ int32_t check(fml_ctx* ctx, const Params& p, int32_t form) {
   return FML_OK;
 }
 
-template <int CW, int SEG, bool GATED, bool BWD>
+template <int WARPS, int LANES, int VEC, int SEG, bool GATED, bool BWD, bool AHEAD, bool TEAM>
 int32_t launch_scan(fml_ctx* ctx, Params& p, int cluster) {
-  p.ctiles = (p.dim + CW - 1) / CW;
+  p.ctiles = (p.dim + LANES * VEC - 1) / (LANES * VEC);
   p.cluster = cluster;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((long long)p.n_seq * p.ctiles * cluster));
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(32 * WARPS);
   cfg.stream = ctx->stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim = {(unsigned)cluster, 1, 1};
   cfg.attrs = at;
-  cfg.numAttrs = cluster > 1 ? 1 : 0;
-  FML_CUDA(ctx, cudaLaunchKernelEx(&cfg, scan_kernel<CW, SEG, GATED, BWD>, (const Params)p));
+  cfg.numAttrs = TEAM ? 1 : 0;
+  FML_CUDA(ctx, cudaLaunchKernelEx(&cfg, scan_kernel<WARPS, LANES, VEC, SEG, GATED, BWD, AHEAD, TEAM>, (const Params)p));
   return FML_OK;
+}
+
+// elements that one load may take: rows, row strides and addresses all allow it
+int vector_width(const Params& p) {
+  uintptr_t all = 0;
+  for (const float* q : {p.f, p.x, p.h, p.dy, (const float*)p.out, (const float*)p.df, (const float*)p.dx}) all |= reinterpret_cast<uintptr_t>(q);
+  const long long n = p.dim | p.ss_in | p.ts_in | p.ss_h | p.ts_h;
+  return (all & 15) == 0 && n % 4 == 0 ? 4 : (all & 7) == 0 && n % 2 == 0 ? 2 : 1;
+}
+
+template <int VEC, bool GATED, bool BWD>
+int32_t launch_lanes(fml_ctx* ctx, Params& p) {
+  constexpr int SEG = 16 / VEC;
+  auto units = [&](int lanes) { return (long long)p.n_seq * ((p.dim + lanes * VEC - 1) / (lanes * VEC)); };
+  const int sms = ctx->sm_count;
+  // Channels enough: CTAs of four warps, each over all steps of its channels, rows as wide as leaves four CTAs an SM
+  if (units(32) >= 3 * sms) return launch_scan<4, 32, VEC, SEG, GATED, BWD, true, false>(ctx, p, 1);
+  if (units(16) >= 4 * sms) return launch_scan<4, 16, VEC, SEG, GATED, BWD, true, false>(ctx, p, 1);
+  if (units(8) >= 4 * sms) return launch_scan<4, 8, VEC, SEG, GATED, BWD, true, false>(ctx, p, 1);
+  if (units(8) >= sms) return launch_scan<8, 8, VEC, SEG, GATED, BWD, true, false>(ctx, p, 1);
+  // Few: eight warps, narrow rows, and a cluster along the steps until there are two CTAs an SM
+  constexpr int LONG = BWD ? SEG : 2 * SEG;
+  int cluster = 1;
+  while (cluster < MAX_CLUSTER && units(4) * cluster * 2 <= 2 * sms && 64ll * LONG * cluster < p.seq_len) cluster <<= 1;
+  if (cluster > 1) return launch_scan<8, 4, VEC, LONG, GATED, BWD, false, true>(ctx, p, cluster);
+  return launch_scan<8, 4, VEC, LONG, GATED, BWD, false, false>(ctx, p, 1);
 }
 
 template <bool GATED, bool BWD>
@@ -298,18 +456,10 @@ int32_t launch(fml_ctx* ctx, Params& p) {
     FML_LAUNCH_CHECK(ctx, "step_kernel");
     return FML_OK;
   }
-  constexpr int SEG = BWD ? 8 : 16;
-  // Few channels: narrower tiles and a cluster along the time axis, until there are four CTAs an SM or no more steps to split
-  const long long want = 4ll * ctx->sm_count;
-  int cw = 32;
-  while (cw > 8 && (long long)p.n_seq * ((p.dim + cw - 1) / cw) * MAX_CLUSTER < want) cw >>= 1;
-  const long long units = (long long)p.n_seq * ((p.dim + cw - 1) / cw);
-  const int tile = WARPS * (32 / cw) * SEG;
-  int cluster = 1;
-  while (cluster < MAX_CLUSTER && units * cluster < want && (long long)tile * cluster < p.seq_len) cluster <<= 1;
-  if (cw == 32) return launch_scan<32, SEG, GATED, BWD>(ctx, p, cluster);
-  if (cw == 16) return launch_scan<16, SEG, GATED, BWD>(ctx, p, cluster);
-  return launch_scan<8, SEG, GATED, BWD>(ctx, p, cluster);
+  const int vec = vector_width(p);
+  if (vec == 4) return launch_lanes<4, GATED, BWD>(ctx, p);
+  if (vec == 2) return launch_lanes<2, GATED, BWD>(ctx, p);
+  return launch_lanes<1, GATED, BWD>(ctx, p);
 }
 
 }  // namespace

@@ -1,11 +1,12 @@
 """Gated linear recurrence (fml_gated_recurrence_*, ops, T.gatedRecurrence, GatedRecurrentLayer) against float64.
 
-Bounds from counting roundings, u = 2^-24 each, to first order.  A gate is off by at most 8 u (exponential 4 u, damped in
-the larger of a and 1 - a, the sum, a two-ulp division), a LINEAR one is exact.  However the steps are grouped, a result is
+Bounds from counting roundings, u = 2^-24 each, to first order.  A gate is off by at most (8 + 1.25 |f|) u (the exponential's
+argument, rounded in base 2 with a rounded constant: 1.25 |f| u; the exponential 4 u, the sum 1 u, the reciprocal 2 u, a
+product), a LINEAR one is exact.  However the steps are grouped, a result is
 the recurrence with every decay off by its own error, one product and one sum: with S_t = |a| S_{t-1} + |s x| the recurrence
-of absolute values, the error obeys E_t = |a| E_{t-1} + k u (|a| S_{t-1} + |s x_t|), k = 12 (GATED) or 4 (LINEAR), the joins
+of absolute values, the error obeys E_t = |a| E_{t-1} + k u (|a| S_{t-1} + |s x_t|), k = 4 and, GATED, the gate's, the joins
 of segments, at most one a step, included; 4 u S_t more for the last roundings.  Backward the same with T_t = |dy_t| + C_{t+1},
-C_t = |a| T_t; dx and df are products of G with gates (24 u), and of the difference of two given numbers (2 u of each).
+C_t = |a| T_t; dx and df are products of G with gates (two of them: 2 (k - 4) + 8 u), and of the difference of two given numbers (2 u of each).
 """
 import numpy as np
 import pytest
@@ -20,10 +21,14 @@ def gates(f, form):
         return (1 / (1 + np.exp(-f)), 1 / (1 + np.exp(f))) if form == "gated" else (f, np.ones_like(f))
 
 
+def rounding(f, form):
+    return 12 + 1.25 * np.abs(np.nan_to_num(f.astype(np.float64), posinf=80, neginf=80)) if form == "gated" else np.full(f.shape, 4.0)
+
+
 def forward64(f, x, h0, lens, form):
     """[n_seq, seq_len, dim] -> h, its bound, the last state, its bound."""
     a, s = gates(f, form)
-    k = 12 if form == "gated" else 4
+    k = rounding(f, form)
     x = x.astype(np.float64)
     state = h0.astype(np.float64).copy()
     S, E = np.abs(state), np.zeros_like(state)
@@ -31,7 +36,7 @@ def forward64(f, x, h0, lens, form):
     for t in range(x.shape[1]):
         on = (t < lens)[:, None]
         add, dec = s[:, t] * x[:, t], np.abs(a[:, t])
-        E = np.where(on, dec * E + k * U * (dec * S + np.abs(add)), E)
+        E = np.where(on, dec * E + k[:, t] * U * (dec * S + np.abs(add)), E)
         S = np.where(on, dec * S + np.abs(add), S)
         state = np.where(on, a[:, t] * state + add, state)
         h[:, t], bound[:, t] = state, E + 4 * U * S
@@ -41,7 +46,7 @@ def forward64(f, x, h0, lens, form):
 def backward64(f, x, h0, h, dy, dh_last, lens, form):
     """-> (df, its bound), (dx, its bound), (dh0, its bound), from the given h."""
     a, s = gates(f, form)
-    k = 12 if form == "gated" else 4
+    k = rounding(f, form)
     x, h, dy = x.astype(np.float64), h.astype(np.float64), dy.astype(np.float64)
     before = np.concatenate([h0.astype(np.float64)[:, None], h[:, :-1]], 1)
     c = dh_last.astype(np.float64).copy()
@@ -53,9 +58,9 @@ def backward64(f, x, h0, h, dy, dh_last, lens, form):
         d = before[:, t] - x[:, t] if form == "gated" else before[:, t]
         D = np.abs(before[:, t]) + np.abs(x[:, t]) if form == "gated" else np.abs(d)
         w = a[:, t] * s[:, t] if form == "gated" else np.ones_like(G)
-        dx[:, t], bx[:, t] = s[:, t] * G, s[:, t] * (EG + 24 * U * T)
-        df[:, t], bf[:, t] = G * d * w, w * (np.abs(d) * (EG + 24 * U * T) + 2 * U * D * T)
-        E = np.where(on, np.abs(a[:, t]) * EG + k * U * np.abs(a[:, t]) * T, E)
+        dx[:, t], bx[:, t] = s[:, t] * G, s[:, t] * (EG + 2 * k[:, t] * U * T)
+        df[:, t], bf[:, t] = G * d * w, w * (np.abs(d) * (EG + 2 * k[:, t] * U * T) + 2 * U * D * T)
+        E = np.where(on, np.abs(a[:, t]) * EG + k[:, t] * U * np.abs(a[:, t]) * T, E)
         C = np.where(on, np.abs(a[:, t]) * T, C)
         c = np.where(on, a[:, t] * G, c)
         for v in (df, dx, bf, bx):
