@@ -86,24 +86,36 @@ __global__ void advance_kernel(DeviceStep* d, const HyperIn p) {
   d->h = hyper_at(p, d->t);
 }
 
-// value of a code in units of its scale: with the seven bits under the exponent's place and 2^120, subnormals come out right too
-__device__ __forceinline__ float decode8(uint32_t c) {
-  const float v = __uint_as_float((c & 0x7fu) << 20) * 0x1p120f;
-  return (c & 0x7fu) == 0x7fu ? __uint_as_float(0x7fc00000u) : __uint_as_float(__float_as_uint(v) | (c & 0x80u) << 24);
-}
 __device__ __forceinline__ bool finite_bits(uint32_t b) { return (b & 0x7fffffffu) < 0x7f800000u; }
+
+// four codes in units of their scale
+__device__ __forceinline__ void decode8(uint32_t codes, float* out) {
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    uint32_t h2;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((unsigned short)(codes >> (16 * i))));
+    asm("{\n\t.reg .f16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.f32.f16 %0, l;\n\tcvt.f32.f16 %1, h;\n\t}" : "=f"(out[2 * i]), "=f"(out[2 * i + 1]) : "r"(h2));
+  }
+}
 
 // exponent of the block's scale from the bits of its largest finite absolute value
 __device__ __forceinline__ int scale_exponent(uint32_t amax) { return max((int)((amax + 0x1FFFFFu) >> 23) - 135, -126); }
 
-// `y` = |x| / scale in [0, 448]; values below 2^-6 are moved up by 2^-6, where the steps of 2^-9 are float steps of the same
-// place, and back in the code
+// x / scale, brought down by 2^-120: 2^-6, the format's smallest normal number, becomes float's, so that the float's bits from
+// the twentieth on ARE the code, subnormal or not, and what lies below them is what is rounded away.  Returns those bits with
+// the rounding added, the sign on top.
 template <bool NEAREST>
-__device__ __forceinline__ uint32_t encode8(float y, uint32_t rnd16) {
-  const bool small = y < 0x1p-6f;
-  const uint32_t z = __float_as_uint(small ? y + 0x1p-6f : y);
-  const uint32_t up = NEAREST ? 0x7FFFFu + ((z >> 20) & 1u) : rnd16 << 4;
-  return ((z + up) >> 20) - (small ? 968u : 960u);
+__device__ __forceinline__ uint32_t encode8(float x, float inv_scale, uint32_t rnd16) {
+  const uint32_t z = __float_as_uint(__fmul_rn(__fmul_rn(x, inv_scale), 0x1p-120f));
+  return z + (NEAREST ? 0x7FFFFu + ((z >> 20) & 1u) : rnd16 * 16u);
+}
+// the codes of four encoded numbers
+template <bool SIGNED>
+__device__ __forceinline__ uint32_t pack8(const uint32_t* z) {
+  uint32_t b[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) b[i] = SIGNED ? z[i] << 4 | (z[i] & 0x80000000u) : z[i] << 4;
+  return __byte_perm(__byte_perm(b[0], b[1], 0x0073), __byte_perm(b[2], b[3], 0x0073), 0x5410);
 }
 
 template <bool EIGHT, bool NEAREST, bool ZERO>
@@ -149,32 +161,37 @@ __global__ void __launch_bounds__(32 * WARPS) adamw_kernel(const Item* __restric
     }
   }
   if (dev) h = dev->h;
-  float root[8];
-  uint32_t mmax = 0, rmax = 0;
+  if (EIGHT) {
+#pragma unroll
+    for (int q = 0; q < 2; q++) {
+      decode8(mc[q], mv + 4 * q);
+      decode8(rc[q], vv + 4 * q);
+    }
+  }
+  float root[8], mmax = 0.f, rmax = 0.f, all = 0.f;
 #pragma unroll
   for (int j = 0; j < 8; j++) {
-    float m, v;
+    float m = mv[j], v = vv[j];
     if (EIGHT) {
-      m = __fmul_rn(decode8(mc[j >> 2] >> (8 * (j & 3)) & 0xffu), ms);
-      const float r = __fmul_rn(decode8(rc[j >> 2] >> (8 * (j & 3)) & 0xffu), rs);
-      v = __fmul_rn(r, r);
-    } else {
-      m = mv[j];
-      v = vv[j];
+      m = __fmul_rn(m, ms);
+      v = __fmul_rn(v, rs);
+      v = __fmul_rn(v, v);
     }
     const float gj = __fmul_rn(gv[j], h.gs);
     m = __fadd_rn(__fmul_rn(m, h.b1), __fmul_rn(gj, h.omb1));
     v = __fadd_rn(__fmul_rn(v, h.b2), __fmul_rn(__fmul_rn(gj, gj), h.omb2));
     root[j] = __fsqrt_rn(v);
-    // the quotient to two units in the last place: it moves w by lr times that
-    wv[j] -= __fdividef(h.step * m, fmaf(root[j], h.rc2, h.eps));
+    // the hardware's reciprocal, good to one unit in the last place: it moves w by lr times that
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(fmaf(root[j], h.rc2, h.eps)));
+    wv[j] -= h.step * m * inv;
     wv[j] -= h.decay * wv[j];
     mv[j] = m;
     vv[j] = v;
     if (EIGHT) {
-      const uint32_t mb = __float_as_uint(m) & 0x7fffffffu, rb = __float_as_uint(root[j]);
-      mmax = max(mmax, finite_bits(mb) ? mb : 0u);
-      rmax = max(rmax, finite_bits(rb) ? rb : 0u);
+      mmax = fmaxf(mmax, fabsf(m));
+      rmax = fmaxf(rmax, root[j]);
+      all += fabsf(m) + root[j];   // not finite if one of them is not
     }
   }
   if (vec) {
@@ -201,21 +218,44 @@ __global__ void __launch_bounds__(32 * WARPS) adamw_kernel(const Item* __restric
     }
     return;
   }
-  const int me = scale_exponent(__reduce_max_sync(0xffffffffu, mmax)), re = scale_exponent(__reduce_max_sync(0xffffffffu, rmax));
+  // A block with a number that is not finite leaves it out of its scale and makes its code NaN (fmaxf has passed over NaN).
+  const bool odd = __any_sync(0xffffffffu, !(all < INFINITY));
+  if (odd) {
+    mmax = rmax = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      if (finite_bits(__float_as_uint(mv[j]))) mmax = fmaxf(mmax, fabsf(mv[j]));
+      if (finite_bits(__float_as_uint(root[j]))) rmax = fmaxf(rmax, root[j]);
+    }
+  }
+  const int me = scale_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(mmax)));
+  const int re = scale_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(rmax)));
   const float mi = __int_as_float((127 - me) << 23), ri = __int_as_float((127 - re) << 23);
   const uint32_t key = NEAREST ? 0u : mix32(h.key + (uint32_t)b * 0x9E3779B1u);
-  uint32_t mo[2] = {0, 0}, ro[2] = {0, 0};
+  uint32_t mo[2], ro[2];
 #pragma unroll
-  for (int j = 0; j < 8; j++) {
-    const uint32_t word = NEAREST ? 0u : mix32(key + (j >> 2) * 128 + 4 * lane + (j & 3));
-    const uint32_t mb = __float_as_uint(mv[j]), rb = __float_as_uint(root[j]);
-    uint32_t cm = encode8<NEAREST>(__fmul_rn(fabsf(mv[j]), mi), word >> 16);
-    uint32_t cr = encode8<NEAREST>(__fmul_rn(root[j], ri), word & 0xffffu);
-    cm = (finite_bits(mb) ? cm : 0x7fu) | (mb >> 31) << 7;
-    if (cr == 0 && root[j] > 0.f) cr = 1;
-    cr = finite_bits(rb) ? cr : 0x7fu;
-    mo[j >> 2] |= cm << (8 * (j & 3));
-    ro[j >> 2] |= cr << (8 * (j & 3));
+  for (int q = 0; q < 2; q++) {
+    uint32_t zm[4], zr[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const uint32_t word = NEAREST ? 0u : mix32(key + q * 128 + 4 * lane + i);
+      zm[i] = encode8<NEAREST>(mv[4 * q + i], mi, word >> 16);
+      zr[i] = encode8<NEAREST>(root[4 * q + i], ri, word & 0xffffu);
+    }
+    mo[q] = pack8<true>(zm);
+    ro[q] = pack8<false>(zr);
+    if ((ro[q] - 0x01010101u) & 0x80808080u) {        // some code is 0: a positive root keeps the smallest one
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if ((ro[q] >> (8 * i) & 0xffu) == 0 && root[4 * q + i] > 0.f) ro[q] |= 1u << (8 * i);
+    }
+    if (odd) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if (!finite_bits(__float_as_uint(mv[4 * q + i]))) mo[q] |= 0xffu << (8 * i);
+        if (!finite_bits(__float_as_uint(root[4 * q + i]))) ro[q] = (ro[q] & ~(0xffu << (8 * i))) | 0x7fu << (8 * i);
+      }
+    }
   }
   uint32_t* mw = reinterpret_cast<uint32_t*>(mbuf) + b * (BLOCK / 4);
   uint32_t* rw = reinterpret_cast<uint32_t*>(vbuf) + b * (BLOCK / 4);
@@ -343,8 +383,8 @@ int32_t fml_adamw_plan_step(fml_ctx* ctx, int32_t plan_id, int32_t lane, double 
   FML_ENTER(ctx);
   FML_REQUIRE(ctx, plan_id >= 0 && plan_id < (int32_t)ctx->adamw_plans.size() && ctx->adamw_plans[plan_id], "fml_adamw_plan_step: unknown plan");
   FML_REQUIRE(ctx, beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, "fml_adamw_plan_step: betas must be in [0, 1)");
-  FML_REQUIRE(ctx, eps > 0 && isfinite(eps) && isfinite(lr) && isfinite(weight_decay) && isfinite(grad_scale),
-              "fml_adamw_plan_step: hyper-parameters must be finite, eps positive");
+  FML_REQUIRE(ctx, eps >= 1e-37 && isfinite(eps) && isfinite(lr) && isfinite(weight_decay) && isfinite(grad_scale),
+              "fml_adamw_plan_step: hyper-parameters must be finite, eps at least 1e-37");
   FML_REQUIRE(ctx, t >= 0, "fml_adamw_plan_step: t must be >= 1, or 0 for the plan's own counter");
   cudaStream_t s;
   const int32_t rc = fml_any_stream(ctx, lane, &s);

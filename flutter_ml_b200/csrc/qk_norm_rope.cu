@@ -14,7 +14,9 @@
 // is the reduction.  A warp takes 32 / lanes heads of a row at once, queries and keys alike, and its next items' loads go
 // out before the first is used.  The cosines and sines of a CTA's rows are formed once, into shared memory, for all heads:
 // the angle in turns in double (pos times a frequency keeps no fraction in 24 bits at far positions), its fraction in float.
-// Head widths, row strides or addresses that do not allow float4 run the same steps with one warp a head, pairs of floats.
+// Addresses or row strides that float4 cannot take
+// are read float by float in the same places; head widths and rotated parts that are no multiple of eight run the same steps
+// with one warp a head, pairs of floats.
 // dgain: each CTA leaves its sums in the caller's scratch, a second launch adds them in a fixed order.
 #include <math.h>
 
@@ -35,6 +37,8 @@ struct Side {          // queries or keys
   long long ldx, ldy, ldo;
   const float* gain;
   int heads;
+  uint32_t per_head;   // ceil(2^32 / heads): divides by multiplying
+  int wide;            // which of x (1), dy (2), out (4) can be read or written four floats at a time
 };
 struct Params {
   Side s[2];
@@ -69,43 +73,157 @@ __device__ __forceinline__ float head_sum(float v) {
   return v;
 }
 
-// the lane's eight elements turned by +angle (sign = 1) or back (sign = -1)
-__device__ __forceinline__ void turn8(float* z, const float* c, const float* s, float sign, int interleaved) {
+__device__ __forceinline__ float inv_root(float v) {   // two units in the last place; eps keeps v a normal number
+  float r;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ void load4(float* v, const float* p, bool wide) {
+  if (wide) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p);
+  else
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = p[i];
+}
+__device__ __forceinline__ void store4(float* p, const float* v, bool wide) {
+  if (wide) *reinterpret_cast<float4*>(p) = *reinterpret_cast<const float4*>(v);
+  else
+#pragma unroll
+    for (int i = 0; i < 4; i++) p[i] = v[i];
+}
+
+// A lane's place in a head: four elements from e0 on and four from e1 on; in the rotated part the two hold each other's
+// partners (pairs apart) or two pairs each (neighbouring pairs).
+struct Place {
+  int e0, e1, half, u;
+  bool active, turned;
+};
+
+// z turned by +angle (sign = 1) or back (sign = -1)
+template <bool INTER>
+__device__ __forceinline__ void turn8(float* z, const float* cosr, const float* sinr, const Place& at, float sign) {
+  float c[4], s[4];
+  if (INTER) {
+    *reinterpret_cast<float2*>(c) = *reinterpret_cast<const float2*>(cosr + 2 * at.u);
+    *reinterpret_cast<float2*>(c + 2) = *reinterpret_cast<const float2*>(cosr + (at.half >> 1) + 2 * at.u);
+    *reinterpret_cast<float2*>(s) = *reinterpret_cast<const float2*>(sinr + 2 * at.u);
+    *reinterpret_cast<float2*>(s + 2) = *reinterpret_cast<const float2*>(sinr + (at.half >> 1) + 2 * at.u);
+  } else {
+    *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(cosr + 4 * at.u);
+    *reinterpret_cast<float4*>(s) = *reinterpret_cast<const float4*>(sinr + 4 * at.u);
+  }
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    const int ia = interleaved ? 2 * i : i, ib = interleaved ? 2 * i + 1 : i + 4;
+    const int ia = INTER ? 2 * i : i, ib = INTER ? 2 * i + 1 : i + 4;
     const float a = z[ia], b = z[ib], sn = sign * s[i];
     z[ia] = a * c[i] - b * sn;
     z[ib] = a * sn + b * c[i];
   }
 }
 
+// The heads of one side (queries or keys) in rows [r0, r0 + n): counted through, HPW of them a warp's item.
+template <int LPH, bool BWD, bool INTER>
+__device__ __forceinline__ void side_heads(const Params& p, const Side& s, long long r0, int n, const float* cosv, const float* sinv,
+                                           const Place& at, const float* gain, float* dg) {
+  constexpr int HPW = 32 / LPH, U = BWD ? 2 : 4;      // heads of an item; items whose loads go out together
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LPH;
+  const int total = n * s.heads, d = p.d;
+  const bool wx = s.wide & 1, wy = s.wide & 2, wo = s.wide & 4;
+  const float inv_d = 1.f / (float)d;
+  const float* x0 = s.x + r0 * s.ldx;
+  const float* y0 = s.dy + r0 * s.ldy;
+  float* o0 = s.out + r0 * s.ldo;
+  for (int it = warp * HPW; it < total; it += WARPS * HPW * U) {
+    float x[U][8], dy[BWD ? U : 1][8];
+    int row[U], col[U];
+#pragma unroll
+    for (int k = 0; k < U; k++) {
+      const int head = it + k * WARPS * HPW + sub;
+      row[k] = s.heads == 1 ? head : (int)__umulhi((uint32_t)head, s.per_head);
+      col[k] = (head - row[k] * s.heads) * d;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        x[k][i] = 0.f;
+        if (BWD) dy[k][i] = 0.f;
+      }
+      if (at.active && head < total) {
+        const float* src = x0 + row[k] * s.ldx + col[k];
+        load4(x[k], src + at.e0, wx);
+        load4(x[k] + 4, src + at.e1, wx);
+        if (BWD) {
+          src = y0 + row[k] * s.ldy + col[k];
+          load4(dy[k], src + at.e0, wy);
+          load4(dy[k] + 4, src + at.e1, wy);
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < U; k++) {
+      const int first = it + k * WARPS * HPW;
+      if (first >= total) break;                      // the same for the whole warp
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; i++) ss = fmaf(x[k][i], x[k][i], ss);
+      const float rstd = inv_root(fmaf(head_sum<LPH>(ss), inv_d, p.eps));
+      const int table = min(row[k], n - 1) * at.half;
+      float z[8];
+      if (!BWD) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) z[i] = x[k][i] * rstd * gain[i];
+        if (at.turned) turn8<INTER>(z, cosv + table, sinv + table, at, 1.f);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) z[i] = dy[k][i];
+        if (at.turned) turn8<INTER>(z, cosv + table, sinv + table, at, -1.f);
+        float dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          x[k][i] *= rstd;
+          dg[i] = fmaf(z[i], x[k][i], dg[i]);
+          z[i] *= gain[i];
+          dot = fmaf(z[i], x[k][i], dot);
+        }
+        dot = head_sum<LPH>(dot) * inv_d;
+#pragma unroll
+        for (int i = 0; i < 8; i++) z[i] = rstd * (z[i] - x[k][i] * dot);
+      }
+      if (at.active && first + sub < total) {
+        float* dst = o0 + row[k] * s.ldo + col[k];
+        if (BWD && p.accumulate) {
+          float old[8];
+          load4(old, dst + at.e0, wo);
+          load4(old + 4, dst + at.e1, wo);
+#pragma unroll
+          for (int i = 0; i < 8; i++) z[i] += old[i];
+        }
+        store4(dst + at.e0, z, wo);
+        store4(dst + at.e1, z + 4, wo);
+      }
+    }
+  }
+}
+
 template <int LPH, bool BWD, bool INTER>
 __global__ void __launch_bounds__(THREADS) qk_vec_kernel(const Params p) {
-  extern __shared__ float sm[];
-  constexpr int HPW = 32 / LPH;                       // heads of a warp's item
-  constexpr int U = BWD ? 2 : 4;                      // items whose loads go out together
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int u = lane % LPH, sub = lane / LPH;
-  const int half = p.rot >> 1, d = p.d;
+  extern __shared__ __align__(16) float sm[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LPH;
+  const int d = p.d;
+  Place at;
+  at.u = lane % LPH;
+  at.half = p.rot >> 1;
+  at.active = at.u < (d >> 3);
+  at.turned = at.u < (p.rot >> 3);
+  at.e0 = at.turned ? 4 * at.u : p.rot + 4 * (at.u - (p.rot >> 3));
+  at.e1 = at.turned ? 4 * at.u + at.half : at.e0 + ((d - p.rot) >> 1);
   float* cosv = sm;
-  float* sinv = sm + p.rows_cta * half;
-  const int total = p.s[0].heads + p.s[1].heads;
-  const int groups = (total + HPW - 1) / HPW;
-  // the lane's place in a head: e0, e1 (four elements each); a rotated unit takes both halves of its pairs
-  const bool active = u < (d >> 3);
-  const bool turned = u < (p.rot >> 3);
-  const int e0 = turned ? 4 * u : p.rot + 4 * (u - (p.rot >> 3));
-  const int e1 = turned ? 4 * u + half : e0 + ((d - p.rot) >> 1);
+  float* sinv = sm + p.rows_cta * at.half;
   float gain[2][8], dg[2][8];
 #pragma unroll
   for (int t = 0; t < 2; t++)
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      gain[t][i] = active && p.s[t].gain ? p.s[t].gain[(i < 4 ? e0 : e1) + (i & 3)] : 1.f;
+      gain[t][i] = at.active && p.s[t].gain ? p.s[t].gain[(i < 4 ? at.e0 : at.e1) + (i & 3)] : 1.f;
       dg[t][i] = 0.f;
     }
-  const float inv_d = 1.f / (float)d;
   const long long steps = (p.rows + p.rows_cta - 1) / p.rows_cta;
   for (long long st = blockIdx.x; st < steps; st += gridDim.x) {
     const long long r0 = st * p.rows_cta;
@@ -113,96 +231,8 @@ __global__ void __launch_bounds__(THREADS) qk_vec_kernel(const Params p) {
     __syncthreads();                                  // the table of the step before has been read
     angles(p, r0, n, cosv, sinv);
     __syncthreads();
-    const int items = n * groups;
-    for (int it0 = warp; it0 < items; it0 += WARPS * U) {
-      float x[U][8], dy[BWD ? U : 1][8];
-#pragma unroll
-      for (int k = 0; k < U; k++) {
-        const int it = it0 + k * WARPS;
-        const int r = it / groups, head = (it - r * groups) * HPW + sub;
-        const bool on = it < items && active && head < total;
-        const bool key = head >= p.s[0].heads;
-        const Side& s = p.s[key ? 1 : 0];
-        const int hh = key ? head - p.s[0].heads : head;
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-        if (on) {
-          const float* src = s.x + (r0 + r) * s.ldx + (long long)hh * d;
-          a = *reinterpret_cast<const float4*>(src + e0);
-          b = *reinterpret_cast<const float4*>(src + e1);
-        }
-        reinterpret_cast<float4*>(x[k])[0] = a;
-        reinterpret_cast<float4*>(x[k])[1] = b;
-        if (BWD) {
-          a = b = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (on) {
-            const float* src = s.dy + (r0 + r) * s.ldy + (long long)hh * d;
-            a = *reinterpret_cast<const float4*>(src + e0);
-            b = *reinterpret_cast<const float4*>(src + e1);
-          }
-          reinterpret_cast<float4*>(dy[k])[0] = a;
-          reinterpret_cast<float4*>(dy[k])[1] = b;
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < U; k++) {
-        const int it = it0 + k * WARPS;
-        if (it >= items) break;                       // the same for the whole warp
-        const int r = it / groups, head = (it - r * groups) * HPW + sub;
-        const bool on = active && head < total;
-        const bool key = head >= p.s[0].heads;
-        const Side& s = p.s[key ? 1 : 0];
-        const int hh = key ? head - p.s[0].heads : head;
-        float c[4], sn[4];
-        if (turned) {
-          if (INTER) {
-            *reinterpret_cast<float2*>(c) = *reinterpret_cast<const float2*>(cosv + r * half + 2 * u);
-            *reinterpret_cast<float2*>(c + 2) = *reinterpret_cast<const float2*>(cosv + r * half + (half >> 1) + 2 * u);
-            *reinterpret_cast<float2*>(sn) = *reinterpret_cast<const float2*>(sinv + r * half + 2 * u);
-            *reinterpret_cast<float2*>(sn + 2) = *reinterpret_cast<const float2*>(sinv + r * half + (half >> 1) + 2 * u);
-          } else {
-            *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(cosv + r * half + 4 * u);
-            *reinterpret_cast<float4*>(sn) = *reinterpret_cast<const float4*>(sinv + r * half + 4 * u);
-          }
-        }
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) ss = fmaf(x[k][i], x[k][i], ss);
-        const float rstd = 1.f / sqrtf(fmaf(head_sum<LPH>(ss), inv_d, p.eps));
-        float z[8];
-        if (!BWD) {
-#pragma unroll
-          for (int i = 0; i < 8; i++) z[i] = x[k][i] * rstd * (key ? gain[1][i] : gain[0][i]);
-          if (turned) turn8(z, c, sn, 1.f, INTER);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; i++) z[i] = dy[k][i];
-          if (turned) turn8(z, c, sn, -1.f, INTER);
-          float dot = 0.f;
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const float xh = x[k][i] * rstd, dgi = z[i] * xh;
-            if (key) dg[1][i] += dgi; else dg[0][i] += dgi;
-            z[i] *= key ? gain[1][i] : gain[0][i];
-            dot = fmaf(z[i], xh, dot);
-            x[k][i] = xh;
-          }
-          dot = head_sum<LPH>(dot) * inv_d;
-#pragma unroll
-          for (int i = 0; i < 8; i++) z[i] = rstd * (z[i] - x[k][i] * dot);
-        }
-        if (on) {
-          float* dst = s.out + (r0 + r) * s.ldo + (long long)hh * d;
-          float4 a = reinterpret_cast<float4*>(z)[0], b = reinterpret_cast<float4*>(z)[1];
-          if (BWD && p.accumulate) {
-            const float4 oa = *reinterpret_cast<const float4*>(dst + e0), ob = *reinterpret_cast<const float4*>(dst + e1);
-            a.x += oa.x; a.y += oa.y; a.z += oa.z; a.w += oa.w;
-            b.x += ob.x; b.y += ob.y; b.z += ob.z; b.w += ob.w;
-          }
-          *reinterpret_cast<float4*>(dst + e0) = a;
-          *reinterpret_cast<float4*>(dst + e1) = b;
-        }
-      }
-    }
+    side_heads<LPH, BWD, INTER>(p, p.s[0], r0, n, cosv, sinv, at, gain[0], dg[0]);
+    side_heads<LPH, BWD, INTER>(p, p.s[1], r0, n, cosv, sinv, at, gain[1], dg[1]);
   }
   if (!BWD || !p.parts) return;
   // the CTA's sums: over the warp's heads, then over the warps, in a fixed order
@@ -214,7 +244,7 @@ __global__ void __launch_bounds__(THREADS) qk_vec_kernel(const Params p) {
       float v = dg[t][i];
 #pragma unroll
       for (int o = LPH; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (sub == 0 && active) sm[(warp * 2 + t) * d + (i < 4 ? e0 : e1) + (i & 3)] = v;
+      if (sub == 0 && at.active) sm[(warp * 2 + t) * d + (i < 4 ? at.e0 : at.e1) + (i & 3)] = v;
     }
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * d; i += THREADS) {
@@ -281,7 +311,7 @@ __global__ void __launch_bounds__(THREADS) qk_pair_kernel(const Params p) {
       float ss = 0.f;
 #pragma unroll
       for (int j = 0; j < SLOTS; j++) ss = fmaf(xa[j], xa[j], fmaf(xb[j], xb[j], ss));
-      const float rstd = 1.f / sqrtf(fmaf(head_sum<32>(ss), inv_d, p.eps));
+      const float rstd = inv_root(fmaf(head_sum<32>(ss), inv_d, p.eps));
       float dot = 0.f;
 #pragma unroll
       for (int j = 0; j < SLOTS; j++) {
@@ -374,10 +404,10 @@ bool same(const float* a, long long lda, const float* b, long long ldb) { return
 
 int32_t check(fml_ctx* ctx, const Params& p, double base) {
   FML_REQUIRE(ctx, p.rows >= 0 && p.d >= 1 && p.d <= MAX_D, "fml_qk_norm_rope: d_head must be 1 .. 256");
-  FML_REQUIRE(ctx, p.s[0].heads >= 1 && p.s[1].heads >= 0 && p.s[0].heads <= (1 << 20) && p.s[1].heads <= (1 << 20), "fml_qk_norm_rope: bad number of heads");
+  FML_REQUIRE(ctx, p.s[0].heads >= 1 && p.s[1].heads >= 0 && p.s[0].heads <= 32768 && p.s[1].heads <= 32768, "fml_qk_norm_rope: bad number of heads");
   FML_REQUIRE(ctx, p.rot >= 0 && p.rot <= p.d && p.rot % 2 == 0, "fml_qk_norm_rope: rot_dim must be even, 0 .. d_head");
   FML_REQUIRE(ctx, p.rot == 0 || (base > 0 && isfinite(base)), "fml_qk_norm_rope: base must be positive");
-  FML_REQUIRE(ctx, p.eps > 0 && isfinite(p.eps), "fml_qk_norm_rope: eps must be positive");
+  FML_REQUIRE(ctx, p.eps >= 1e-37f && isfinite(p.eps), "fml_qk_norm_rope: eps must be 1e-37 or more");
   FML_REQUIRE(ctx, p.seq_len >= 0, "fml_qk_norm_rope: bad seq_len");
   for (int t = 0; t < 2; t++) {
     const Side& s = p.s[t];
@@ -405,12 +435,12 @@ int32_t check(fml_ctx* ctx, const Params& p, double base) {
   return FML_OK;
 }
 
-bool can_vec(const Params& p) {
-  if (p.d % 8 || p.rot % 8) return false;   // rest of the head: a multiple of 8 too
-  for (int t = 0; t < 2; t++) {
-    const Side& s = p.s[t];
-    if (s.heads == 0) continue;
-    if (!al16(s.x) || !al16(s.out) || s.ldx % 4 || s.ldo % 4 || (s.dy && (!al16(s.dy) || s.ldy % 4))) return false;
+// Whether heads can be shared out by eights; and what the lanes need to know for that
+bool can_vec(Params& p) {
+  if (p.d % 8 || p.rot % 8) return false;   // the rest of the head is a multiple of 8 then too
+  for (Side& s : p.s) {
+    s.per_head = s.heads > 1 ? (uint32_t)(((1ull << 32) + s.heads - 1) / s.heads) : 0;   // exact below 2^32 / heads
+    s.wide = (al16(s.x) && s.ldx % 4 == 0 ? 1 : 0) | (al16(s.dy) && s.ldy % 4 == 0 ? 2 : 0) | (al16(s.out) && s.ldo % 4 == 0 ? 4 : 0);
   }
   return true;
 }
@@ -426,7 +456,7 @@ int32_t launch(fml_ctx* ctx, Params& p, int* grid_out) {
   const bool vec = can_vec(p);
   const int lph = p.d <= 32 ? 4 : p.d <= 64 ? 8 : p.d <= 128 ? 16 : 32;
   const int total = p.s[0].heads + p.s[1].heads;
-  const int items = vec ? (total + 32 / lph - 1) / (32 / lph) : total;   // a row's
+  const int items = vec ? std::max(1, total / (32 / lph)) : total;   // a row's
   // rows of a CTA's step: 64 items give every warp eight, and the angles are formed by all threads; fewer rows where
   // that would leave SMs without work
   long long rc = std::max(1, std::min(16, 64 / items));

@@ -359,7 +359,7 @@ int32_t fml_adamw_plan_create(fml_ctx* ctx, int32_t n, float* const* w, float* c
  * t = 0 counts the plan's steps on the device, so that every replay of a recorded step advances the count.  grad_scale
  * multiplies g first; zero_grad != 0 clears g in the same pass.  seed concerns 8-bit states only: negative rounds to the
  * nearest code, any other value rounds up or down at random with the probabilities that keep the mean, from a generator
- * over (seed, t, block, element) - the same call gives the same bits.  eps must be positive, betas in [0, 1). */
+ * over (seed, t, block, element) - the same call gives the same bits.  eps must be 1e-37 or more, betas in [0, 1). */
 int32_t fml_adamw_plan_step(fml_ctx* ctx, int32_t plan_id, int32_t lane, double lr, double beta1, double beta2, double eps,
                             double weight_decay, int32_t t, double grad_scale, int32_t zero_grad, int64_t seed);
 int32_t fml_adamw_plan_destroy(fml_ctx* ctx, int32_t plan_id);
@@ -486,7 +486,7 @@ int32_t fml_attention_bwd(fml_ctx* ctx, const fml_attention_desc* d, const float
  *   pos * base^(-2 i / rot_dim): pairs (i, i + rot_dim / 2), or (2 i, 2 i + 1) when interleaved != 0.
  * pos is positions[row] (device, any sign), or row mod seq_len when positions is NULL (seq_len 0: row).  gain_q and gain_k
  * hold d_head floats, NULL means ones; heads_k may be 0 (k is then ignored) and may differ from heads_q.  d_head is 1 to
- * 256, rot_dim even and 0 to d_head (0: no rotation).  An output may be its own input (same address and stride) and shares
+ * 256, rot_dim even and 0 to d_head (0: no rotation), heads at most 32768, eps 1e-37 or more.  An output may be its own input (same address and stride) and shares
  * nothing else with another buffer.
  * Backward: dq, dk from the forward pass's inputs and the gradients of its outputs, overwritten or added to (accumulate);
  * dgain_q, dgain_k (either may be NULL) are added to, through `scratch` of FML_QK_NORM_ROPE_PARTS * 2 * d_head floats
