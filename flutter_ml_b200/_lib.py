@@ -232,6 +232,9 @@ class DeviceArray:
             pass
 
 
+_PLAIN = frozenset((int, float, type(None)))   # argument types that ctypes takes as they are
+
+
 class Context:
     """One fml_ctx: a device, a stream, a scratch arena."""
 
@@ -405,5 +408,9 @@ class Context:
 
     def call(self, name, *args, launches=1):
         """Call any fml_* entry point that takes the context first; DeviceArrays become addresses."""
-        self.check(getattr(self.lib, name)(self.h, *[_addr(a) if isinstance(a, (DeviceArray, np.ndarray)) else a for a in args]))
+        plain = _PLAIN
+        rc = getattr(self.lib, name)(self.h, *[a.ptr if (t := type(a)) is DeviceArray else a if t in plain else
+                                               _addr(a) if isinstance(a, (DeviceArray, np.ndarray)) else a for a in args])
+        if rc:
+            self.check(rc)
         self.launches += launches

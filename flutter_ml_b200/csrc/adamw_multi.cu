@@ -101,12 +101,20 @@ __device__ __forceinline__ void decode8(uint32_t codes, float* out) {
 // exponent of the block's scale from the bits of its largest finite absolute value
 __device__ __forceinline__ int scale_exponent(uint32_t amax) { return max((int)((amax + 0x1FFFFFu) >> 23) - 135, -126); }
 
-// x / scale, brought down by 2^-120: 2^-6, the format's smallest normal number, becomes float's, so that the float's bits from
-// the twentieth on ARE the code, subnormal or not, and what lies below them is what is rounded away.  Returns those bits with
-// the rounding added, the sign on top.
+// What brings x down to x / scale * 2^-120: then 2^-6, the format's smallest normal number, is float's smallest normal number,
+// and the float's bits from the twentieth on ARE the code, subnormal or not, and those below are what is rounded away.
+// Scales above 2^29 need the power in two parts (`pre` is 1 otherwise).
+struct Down {
+  float pre, by;
+};
+__device__ __forceinline__ Down down(int e) {
+  const int pre = e > 29 ? 120 : 0, rest = -120 - e + pre;   // -149 <= rest <= 6
+  return {pre ? 0x1p-120f : 1.f, rest >= -126 ? __int_as_float((rest + 127) << 23) : __int_as_float(1 << (rest + 149))};
+}
+// those bits with the rounding added, the sign on top
 template <bool NEAREST>
-__device__ __forceinline__ uint32_t encode8(float x, float inv_scale, uint32_t rnd16) {
-  const uint32_t z = __float_as_uint(__fmul_rn(__fmul_rn(x, inv_scale), 0x1p-120f));
+__device__ __forceinline__ uint32_t encode8(float x, const Down& d, uint32_t rnd16) {
+  const uint32_t z = __float_as_uint(__fmul_rn(d.pre != 1.f ? __fmul_rn(x, d.pre) : x, d.by));
   return z + (NEAREST ? 0x7FFFFu + ((z >> 20) & 1u) : rnd16 * 16u);
 }
 // the codes of four encoded numbers
@@ -118,108 +126,125 @@ __device__ __forceinline__ uint32_t pack8(const uint32_t* z) {
   return __byte_perm(__byte_perm(b[0], b[1], 0x0073), __byte_perm(b[2], b[3], 0x0073), 0x5410);
 }
 
-template <bool EIGHT, bool NEAREST, bool ZERO>
-__global__ void __launch_bounds__(32 * WARPS) adamw_kernel(const Item* __restrict__ items, float* __restrict__ mbuf, float* __restrict__ vbuf,
-                                                           long long n_blocks, Hyper h, const DeviceStep* __restrict__ dev) {
+// A warp's block on its way through the registers: eight elements a lane, 4 l .. 4 l + 3 and 128 + 4 l ..
+template <bool EIGHT>
+struct Block {
+  float* w;
+  float* g;
+  long long b;                  // block in the state buffers
+  int n;                        // elements from the block's first to the work item's last; none: no block
+  bool vec;                     // a whole block at addresses that float4 can take
+  float wv[8], gv[8];
+  float mv[EIGHT ? 1 : 8], vv[EIGHT ? 1 : 8];
+  uint32_t mc[EIGHT ? 2 : 1], rc[EIGHT ? 2 : 1];
+  float ms, rs;
+};
+
+template <bool EIGHT>
+__device__ __forceinline__ void load_block(Block<EIGHT>& k, const Item& it, const float* mbuf, const float* vbuf, long long n_blocks) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Item it = items[blockIdx.x];
-  const int n = (int)it.count - warp * BLOCK;   // elements left from this warp's block on
-  if (n <= 0) return;
-  const long long b = (long long)it.block + warp;
-  float* __restrict__ w = it.w + warp * BLOCK;
-  float* __restrict__ g = it.g + warp * BLOCK;
-  const bool vec = n >= BLOCK && ((reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(g)) & 15) == 0;
-  float wv[8], gv[8], mv[8], vv[8];
-  uint32_t mc[2], rc[2];
-  float ms = 0.f, rs = 0.f;
-  if (vec) {
+  k.n = (int)it.count - warp * BLOCK;
+  if (k.n <= 0) return;
+  k.b = (long long)it.block + warp;
+  k.w = it.w + warp * BLOCK;
+  k.g = it.g + warp * BLOCK;
+  k.vec = k.n >= BLOCK && ((reinterpret_cast<uintptr_t>(k.w) | reinterpret_cast<uintptr_t>(k.g)) & 15) == 0;
+  if (k.vec) {
 #pragma unroll
     for (int q = 0; q < 2; q++) {
-      reinterpret_cast<float4*>(wv)[q] = reinterpret_cast<const float4*>(w)[lane + 32 * q];
-      reinterpret_cast<float4*>(gv)[q] = reinterpret_cast<const float4*>(g)[lane + 32 * q];
+      reinterpret_cast<float4*>(k.wv)[q] = reinterpret_cast<const float4*>(k.w)[lane + 32 * q];
+      reinterpret_cast<float4*>(k.gv)[q] = reinterpret_cast<const float4*>(k.g)[lane + 32 * q];
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       const int i = (j >> 2) * 128 + 4 * lane + (j & 3);
-      wv[j] = i < n ? w[i] : 0.f;
-      gv[j] = i < n ? g[i] : 0.f;
+      k.wv[j] = i < k.n ? k.w[i] : 0.f;
+      k.gv[j] = i < k.n ? k.g[i] : 0.f;
     }
   }
   if (EIGHT) {
-    const uint32_t* mw = reinterpret_cast<const uint32_t*>(mbuf) + b * (BLOCK / 4);
-    const uint32_t* rw = reinterpret_cast<const uint32_t*>(vbuf) + b * (BLOCK / 4);
+    const uint32_t* mw = reinterpret_cast<const uint32_t*>(mbuf) + k.b * (BLOCK / 4);
+    const uint32_t* rw = reinterpret_cast<const uint32_t*>(vbuf) + k.b * (BLOCK / 4);
 #pragma unroll
-    for (int q = 0; q < 2; q++) { mc[q] = mw[lane + 32 * q]; rc[q] = rw[lane + 32 * q]; }
-    ms = mbuf[n_blocks * (BLOCK / 4) + b];
-    rs = vbuf[n_blocks * (BLOCK / 4) + b];
+    for (int q = 0; q < 2; q++) { k.mc[q] = mw[lane + 32 * q]; k.rc[q] = rw[lane + 32 * q]; }
+    k.ms = mbuf[n_blocks * (BLOCK / 4) + k.b];
+    k.rs = vbuf[n_blocks * (BLOCK / 4) + k.b];
   } else {
 #pragma unroll
     for (int q = 0; q < 2; q++) {
-      reinterpret_cast<float4*>(mv)[q] = reinterpret_cast<const float4*>(mbuf + b * BLOCK)[lane + 32 * q];
-      reinterpret_cast<float4*>(vv)[q] = reinterpret_cast<const float4*>(vbuf + b * BLOCK)[lane + 32 * q];
+      reinterpret_cast<float4*>(k.mv)[q] = reinterpret_cast<const float4*>(mbuf + k.b * BLOCK)[lane + 32 * q];
+      reinterpret_cast<float4*>(k.vv)[q] = reinterpret_cast<const float4*>(vbuf + k.b * BLOCK)[lane + 32 * q];
     }
   }
-  if (dev) h = dev->h;
+}
+
+template <bool EIGHT, bool NEAREST, bool ZERO>
+__device__ __forceinline__ void update_block(Block<EIGHT>& k, float* mbuf, float* vbuf, long long n_blocks, const Hyper& h) {
+  if (k.n <= 0) return;
+  const int lane = threadIdx.x & 31;
+  float m8[8], v8[8];
   if (EIGHT) {
 #pragma unroll
     for (int q = 0; q < 2; q++) {
-      decode8(mc[q], mv + 4 * q);
-      decode8(rc[q], vv + 4 * q);
+      decode8(k.mc[q], m8 + 4 * q);
+      decode8(k.rc[q], v8 + 4 * q);
     }
   }
+  float* mv = EIGHT ? m8 : k.mv;
+  float* vv = EIGHT ? v8 : k.vv;
   float root[8], mmax = 0.f, rmax = 0.f, all = 0.f;
 #pragma unroll
   for (int j = 0; j < 8; j++) {
     float m = mv[j], v = vv[j];
     if (EIGHT) {
-      m = __fmul_rn(m, ms);
-      v = __fmul_rn(v, rs);
+      m = __fmul_rn(m, k.ms);
+      v = __fmul_rn(v, k.rs);
       v = __fmul_rn(v, v);
     }
-    const float gj = __fmul_rn(gv[j], h.gs);
+    const float gj = __fmul_rn(k.gv[j], h.gs);
     m = __fadd_rn(__fmul_rn(m, h.b1), __fmul_rn(gj, h.omb1));
     v = __fadd_rn(__fmul_rn(v, h.b2), __fmul_rn(__fmul_rn(gj, gj), h.omb2));
     root[j] = __fsqrt_rn(v);
     // the hardware's reciprocal, good to one unit in the last place: it moves w by lr times that
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(fmaf(root[j], h.rc2, h.eps)));
-    wv[j] -= h.step * m * inv;
-    wv[j] -= h.decay * wv[j];
+    k.wv[j] -= h.step * m * inv;
+    k.wv[j] -= h.decay * k.wv[j];
     mv[j] = m;
     vv[j] = v;
     if (EIGHT) {
       mmax = fmaxf(mmax, fabsf(m));
       rmax = fmaxf(rmax, root[j]);
-      all += fabsf(m) + root[j];   // not finite if one of them is not
+      all += k.wv[j];   // NaN if m or the root is
     }
   }
-  if (vec) {
+  if (k.vec) {
 #pragma unroll
     for (int q = 0; q < 2; q++) {
-      reinterpret_cast<float4*>(w)[lane + 32 * q] = reinterpret_cast<float4*>(wv)[q];
-      if (ZERO) reinterpret_cast<float4*>(g)[lane + 32 * q] = make_float4(0.f, 0.f, 0.f, 0.f);
+      reinterpret_cast<float4*>(k.w)[lane + 32 * q] = reinterpret_cast<float4*>(k.wv)[q];
+      if (ZERO) reinterpret_cast<float4*>(k.g)[lane + 32 * q] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
   } else {
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       const int i = (j >> 2) * 128 + 4 * lane + (j & 3);
-      if (i < n) {
-        w[i] = wv[j];
-        if (ZERO) g[i] = 0.f;
+      if (i < k.n) {
+        k.w[i] = k.wv[j];
+        if (ZERO) k.g[i] = 0.f;
       }
     }
   }
   if (!EIGHT) {   // places behind a tensor's last element in its last block: m = v = 0 stays so
 #pragma unroll
     for (int q = 0; q < 2; q++) {
-      reinterpret_cast<float4*>(mbuf + b * BLOCK)[lane + 32 * q] = reinterpret_cast<float4*>(mv)[q];
-      reinterpret_cast<float4*>(vbuf + b * BLOCK)[lane + 32 * q] = reinterpret_cast<float4*>(vv)[q];
+      reinterpret_cast<float4*>(mbuf + k.b * BLOCK)[lane + 32 * q] = reinterpret_cast<float4*>(mv)[q];
+      reinterpret_cast<float4*>(vbuf + k.b * BLOCK)[lane + 32 * q] = reinterpret_cast<float4*>(vv)[q];
     }
     return;
   }
   // A block with a number that is not finite leaves it out of its scale and makes its code NaN (fmaxf has passed over NaN).
-  const bool odd = __any_sync(0xffffffffu, !(all < INFINITY));
+  const bool odd = __any_sync(0xffffffffu, !(fabsf(all) < INFINITY) || mmax == INFINITY || rmax == INFINITY);
   if (odd) {
     mmax = rmax = 0.f;
 #pragma unroll
@@ -230,17 +255,17 @@ __global__ void __launch_bounds__(32 * WARPS) adamw_kernel(const Item* __restric
   }
   const int me = scale_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(mmax)));
   const int re = scale_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(rmax)));
-  const float mi = __int_as_float((127 - me) << 23), ri = __int_as_float((127 - re) << 23);
-  const uint32_t key = NEAREST ? 0u : mix32(h.key + (uint32_t)b * 0x9E3779B1u);
+  const Down md = down(me), rd = down(re);
+  const uint32_t key = NEAREST ? 0u : mix32(h.key + (uint32_t)k.b * 0x9E3779B1u) + 4 * lane;
   uint32_t mo[2], ro[2];
 #pragma unroll
   for (int q = 0; q < 2; q++) {
     uint32_t zm[4], zr[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const uint32_t word = NEAREST ? 0u : mix32(key + q * 128 + 4 * lane + i);
-      zm[i] = encode8<NEAREST>(mv[4 * q + i], mi, word >> 16);
-      zr[i] = encode8<NEAREST>(root[4 * q + i], ri, word & 0xffffu);
+      const uint32_t word = NEAREST ? 0u : mix32(key + (q * 128 + i));
+      zm[i] = encode8<NEAREST>(mv[4 * q + i], md, word >> 16);
+      zr[i] = encode8<NEAREST>(root[4 * q + i], rd, word & 0xffffu);
     }
     mo[q] = pack8<true>(zm);
     ro[q] = pack8<false>(zr);
@@ -257,14 +282,26 @@ __global__ void __launch_bounds__(32 * WARPS) adamw_kernel(const Item* __restric
       }
     }
   }
-  uint32_t* mw = reinterpret_cast<uint32_t*>(mbuf) + b * (BLOCK / 4);
-  uint32_t* rw = reinterpret_cast<uint32_t*>(vbuf) + b * (BLOCK / 4);
+  uint32_t* mw = reinterpret_cast<uint32_t*>(mbuf) + k.b * (BLOCK / 4);
+  uint32_t* rw = reinterpret_cast<uint32_t*>(vbuf) + k.b * (BLOCK / 4);
 #pragma unroll
   for (int q = 0; q < 2; q++) { mw[lane + 32 * q] = mo[q]; rw[lane + 32 * q] = ro[q]; }
   if (lane == 0) {
-    mbuf[n_blocks * (BLOCK / 4) + b] = __int_as_float((me + 127) << 23);
-    vbuf[n_blocks * (BLOCK / 4) + b] = __int_as_float((re + 127) << 23);
+    mbuf[n_blocks * (BLOCK / 4) + k.b] = __int_as_float((me + 127) << 23);
+    vbuf[n_blocks * (BLOCK / 4) + k.b] = __int_as_float((re + 127) << 23);
   }
+}
+
+// One work item a CTA: the loads of the other CTAs of the SM run beside its arithmetic.
+
+
+
+template <bool EIGHT, bool NEAREST, bool ZERO>
+__global__ void __launch_bounds__(32 * WARPS, EIGHT ? 5 : 1) adamw_kernel(const Item* __restrict__ items, float* __restrict__ mbuf, float* __restrict__ vbuf, long long n_blocks, Hyper h, const DeviceStep* __restrict__ dev) {
+  Block<EIGHT> k;
+  load_block(k, items[blockIdx.x], mbuf, vbuf, n_blocks);
+  if (dev) h = dev->h;
+  update_block<EIGHT, NEAREST, ZERO>(k, mbuf, vbuf, n_blocks, h);
 }
 
 int64_t blocks_of(int64_t n) { return (n + BLOCK - 1) / BLOCK; }

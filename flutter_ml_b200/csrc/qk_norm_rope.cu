@@ -29,6 +29,9 @@ namespace {
 constexpr int WARPS = 8, THREADS = 32 * WARPS;
 constexpr int MAX_PARTS = FML_QK_NORM_ROPE_PARTS;   // CTAs of a backward launch, one partial sum each
 constexpr int MAX_D = 256;
+// CTAs an SM: 64 registers a thread forward, 128 backward.  Measured on 16384 rows of 16 + 16 heads of 64, both passes: 129 us;
+// backward with three (80 registers, spills) or four items' loads in flight forward (three CTAs): 140 us.
+constexpr int CTAS_FWD = 4, CTAS_BWD = 2;
 
 struct Side {          // queries or keys
   const float* x;
@@ -46,24 +49,33 @@ struct Params {
   float* parts;        // [CTA][2][d], or NULL when no gain gradient is wanted
   long long rows;
   int seq_len, d, rot, interleaved, accumulate;
-  int rows_cta;        // rows of a CTA's step
+  int rows_cta;        // rows whose angles a CTA forms at once
   double kexp;         // -2 log2(base) / rot
   float eps;
 };
 
-// cosines and sines of rows [r0, r0 + n) into tab[row][rot / 2] and tab2[row][rot / 2]
-__device__ __forceinline__ void angles(const Params& p, long long r0, int n, float* cosv, float* sinv) {
+// Turns a position of the pairs, in double: once a CTA (the power costs as much as ten sines)
+__device__ __forceinline__ void frequencies(const Params& p, double* freq) {
+  for (int j = threadIdx.x; j < p.rot >> 1; j += THREADS) freq[j] = exp2(p.kexp * j) * 0.15915494309189533577;
+}
+// cosines and sines of rows [r0, r0 + n), rot / 2 each a row
+__device__ __forceinline__ void angles(const Params& p, const double* freq, long long r0, int n, float* cosv, float* sinv) {
   const int half = p.rot >> 1;
   for (int i = threadIdx.x; i < n * half; i += THREADS) {
     const int r = i / half, j = i - r * half;
     const long long row = r0 + r;
-    const double pos = p.pos ? (double)p.pos[row] : (double)(p.seq_len > 0 ? row % p.seq_len : row);
-    const double turns = pos * (exp2(p.kexp * j) * 0.15915494309189533577);
+    const double turns = (p.pos ? (double)p.pos[row] : (double)(p.seq_len > 0 ? row % p.seq_len : row)) * freq[j];
     float s, c;
     sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
     cosv[i] = c;
     sinv[i] = s;
   }
+}
+
+// first row of CTA b's share: neighbouring rows, the shares equal to a row
+__device__ __forceinline__ long long share(long long rows, unsigned b) {
+  const long long each = rows / gridDim.x, more = rows - each * gridDim.x;
+  return each * b + min((long long)b, more);
 }
 
 template <int LPH>
@@ -123,8 +135,8 @@ __device__ __forceinline__ void turn8(float* z, const float* cosr, const float* 
 // The heads of one side (queries or keys) in rows [r0, r0 + n): counted through, HPW of them a warp's item.
 template <int LPH, bool BWD, bool INTER>
 __device__ __forceinline__ void side_heads(const Params& p, const Side& s, long long r0, int n, const float* cosv, const float* sinv,
-                                           const Place& at, const float* gain, float* dg) {
-  constexpr int HPW = 32 / LPH, U = BWD ? 2 : 4;      // heads of an item; items whose loads go out together
+                                           const Place& at, float* dg) {
+  constexpr int HPW = 32 / LPH, U = 2;                // heads of an item; items whose loads go out together
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LPH;
   const int total = n * s.heads, d = p.d;
   const bool wx = s.wide & 1, wy = s.wide & 2, wo = s.wide & 4;
@@ -132,6 +144,9 @@ __device__ __forceinline__ void side_heads(const Params& p, const Side& s, long 
   const float* x0 = s.x + r0 * s.ldx;
   const float* y0 = s.dy + r0 * s.ldy;
   float* o0 = s.out + r0 * s.ldo;
+  float gain[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) gain[i] = at.active && s.gain ? __ldg(s.gain + (i < 4 ? at.e0 : at.e1) + (i & 3)) : 1.f;
   for (int it = warp * HPW; it < total; it += WARPS * HPW * U) {
     float x[U][8], dy[BWD ? U : 1][8];
     int row[U], col[U];
@@ -203,7 +218,7 @@ __device__ __forceinline__ void side_heads(const Params& p, const Side& s, long 
 }
 
 template <int LPH, bool BWD, bool INTER>
-__global__ void __launch_bounds__(THREADS) qk_vec_kernel(const Params p) {
+__global__ void __launch_bounds__(THREADS, BWD ? CTAS_BWD : CTAS_FWD) qk_vec_kernel(const Params p) {
   extern __shared__ __align__(16) float sm[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LPH;
   const int d = p.d;
@@ -214,25 +229,23 @@ __global__ void __launch_bounds__(THREADS) qk_vec_kernel(const Params p) {
   at.turned = at.u < (p.rot >> 3);
   at.e0 = at.turned ? 4 * at.u : p.rot + 4 * (at.u - (p.rot >> 3));
   at.e1 = at.turned ? 4 * at.u + at.half : at.e0 + ((d - p.rot) >> 1);
+  __shared__ double freq[MAX_D / 2];
+  frequencies(p, freq);
   float* cosv = sm;
   float* sinv = sm + p.rows_cta * at.half;
-  float gain[2][8], dg[2][8];
+  float dg[2][8];
 #pragma unroll
   for (int t = 0; t < 2; t++)
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      gain[t][i] = at.active && p.s[t].gain ? p.s[t].gain[(i < 4 ? at.e0 : at.e1) + (i & 3)] : 1.f;
-      dg[t][i] = 0.f;
-    }
-  const long long steps = (p.rows + p.rows_cta - 1) / p.rows_cta;
-  for (long long st = blockIdx.x; st < steps; st += gridDim.x) {
-    const long long r0 = st * p.rows_cta;
-    const int n = (int)min((long long)p.rows_cta, p.rows - r0);
+    for (int i = 0; i < 8; i++) dg[t][i] = 0.f;
+  const long long last = share(p.rows, blockIdx.x + 1);
+  for (long long r0 = share(p.rows, blockIdx.x); r0 < last; r0 += p.rows_cta) {
+    const int n = (int)min((long long)p.rows_cta, last - r0);
     __syncthreads();                                  // the table of the step before has been read
-    angles(p, r0, n, cosv, sinv);
+    angles(p, freq, r0, n, cosv, sinv);
     __syncthreads();
-    side_heads<LPH, BWD, INTER>(p, p.s[0], r0, n, cosv, sinv, at, gain[0], dg[0]);
-    side_heads<LPH, BWD, INTER>(p, p.s[1], r0, n, cosv, sinv, at, gain[1], dg[1]);
+    side_heads<LPH, BWD, INTER>(p, p.s[0], r0, n, cosv, sinv, at, dg[0]);
+    side_heads<LPH, BWD, INTER>(p, p.s[1], r0, n, cosv, sinv, at, dg[1]);
   }
   if (!BWD || !p.parts) return;
   // the CTA's sums: over the warp's heads, then over the warps, in a fixed order
@@ -262,6 +275,8 @@ __global__ void __launch_bounds__(THREADS) qk_pair_kernel(const Params p) {
   constexpr int SLOTS = MAX_D / 64;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int half = p.rot >> 1, d = p.d;
+  __shared__ double freq[MAX_D / 2];
+  frequencies(p, freq);
   float* cosv = sm;
   float* sinv = sm + p.rows_cta * half;
   const int total = p.s[0].heads + p.s[1].heads;
@@ -281,12 +296,11 @@ __global__ void __launch_bounds__(THREADS) qk_pair_kernel(const Params p) {
     dg[0][j][0] = dg[0][j][1] = dg[1][j][0] = dg[1][j][1] = 0.f;
   }
   const float inv_d = 1.f / (float)d;
-  const long long steps = (p.rows + p.rows_cta - 1) / p.rows_cta;
-  for (long long st = blockIdx.x; st < steps; st += gridDim.x) {
-    const long long r0 = st * p.rows_cta;
-    const int n = (int)min((long long)p.rows_cta, p.rows - r0);
+  const long long last = share(p.rows, blockIdx.x + 1);
+  for (long long r0 = share(p.rows, blockIdx.x); r0 < last; r0 += p.rows_cta) {
+    const int n = (int)min((long long)p.rows_cta, last - r0);
     __syncthreads();
-    angles(p, r0, n, cosv, sinv);
+    angles(p, freq, r0, n, cosv, sinv);
     __syncthreads();
     for (int it = warp; it < n * total; it += WARPS) {
       const int r = it / total, head = it - r * total;
@@ -371,21 +385,30 @@ __global__ void __launch_bounds__(THREADS) qk_pair_kernel(const Params p) {
   }
 }
 
-// dgain += the CTAs' sums, 32 columns a block, in a fixed order
-__global__ void __launch_bounds__(THREADS) qk_gain_kernel(const float* __restrict__ parts, int n_parts, int d, float* dgain_q, float* dgain_k) {
-  __shared__ float red[WARPS][32];
+// dgain += the CTAs' sums, 32 columns a block, in a fixed order.  32 warps, so that a thread's loads are one trip to memory:
+// with eight it took 10 us.
+__global__ void __launch_bounds__(1024) qk_gain_kernel(const float* __restrict__ parts, int n_parts, int d, float* dgain_q, float* dgain_k) {
+  __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
-  float v = 0.f;
-  if (i < 2 * d) {
-#pragma unroll 8
-    for (int c = warp; c < n_parts; c += WARPS) v += parts[(long long)c * 2 * d + i];
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // the launch overlaps the main kernel's end, the reading does not
+  constexpr int PER = (MAX_PARTS + 31) / 32;
+  float v[PER], sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < PER; k++) {
+    const int c = warp + 32 * k;
+    v[k] = i < 2 * d && c < n_parts ? parts[(long long)c * 2 * d + i] : 0.f;
   }
-  red[warp][lane] = v;
+#pragma unroll
+  for (int k = 0; k < PER; k++) sum += v[k];
+  red[lane][warp] = sum;
   __syncthreads();
-  if (warp != 0 || i >= 2 * d) return;
-  for (int w = 1; w < WARPS; w++) v += red[w][lane];
-  float* dst = i < d ? dgain_q : dgain_k;
-  if (dst) dst[i < d ? i : i - d] += v;
+  sum = red[warp][lane];                              // column `warp` of the block, the warps' sums across the lanes
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  const int col = blockIdx.x * 32 + warp;
+  if (lane != 0 || col >= 2 * d) return;
+  float* dst = col < d ? dgain_q : dgain_k;
+  if (dst) dst[col < d ? col : col - d] += sum;
 }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -455,16 +478,12 @@ template <bool BWD>
 int32_t launch(fml_ctx* ctx, Params& p, int* grid_out) {
   const bool vec = can_vec(p);
   const int lph = p.d <= 32 ? 4 : p.d <= 64 ? 8 : p.d <= 128 ? 16 : 32;
-  const int total = p.s[0].heads + p.s[1].heads;
-  const int items = vec ? std::max(1, total / (32 / lph)) : total;   // a row's
-  // rows of a CTA's step: 64 items give every warp eight, and the angles are formed by all threads; fewer rows where
-  // that would leave SMs without work
-  long long rc = std::max(1, std::min(16, 64 / items));
-  while (rc > 1 && (p.rows + rc - 1) / rc < 2ll * ctx->sm_count) rc >>= 1;
-  p.rows_cta = (int)rc;
-  const long long steps = (p.rows + rc - 1) / rc;
-  const int grid = (int)std::min<long long>(steps, BWD ? std::min(MAX_PARTS, 4 * ctx->sm_count) : 8ll * ctx->sm_count);
-  const size_t smem = std::max<size_t>((size_t)rc * p.rot * 4, BWD ? (size_t)WARPS * 2 * p.d * 4 : 0);   // at most 16 KB
+  const int fit = ctx->sm_count * (BWD ? CTAS_BWD : CTAS_FWD);
+  const int grid = (int)std::min<long long>({p.rows, fit, BWD ? MAX_PARTS : fit});
+  // rows whose angles are formed at once: a table of 32 KB at most, and no more than the CTA has
+  p.rows_cta = (int)std::min<long long>(std::min(32, 8192 / std::max(p.rot, 1)), (p.rows + grid - 1) / grid);
+  const int rc = p.rows_cta;
+  const size_t smem = std::max<size_t>((size_t)rc * p.rot * 4, BWD ? (size_t)WARPS * 2 * p.d * 4 : 0);   // at most 32 KB
   if (!vec) qk_pair_kernel<BWD><<<grid, THREADS, smem, ctx->stream>>>(p);
   else if (lph == 4) launch_vec<4, BWD>(p, grid, smem, ctx->stream);
   else if (lph == 8) launch_vec<8, BWD>(p, grid, smem, ctx->stream);
@@ -519,8 +538,16 @@ int32_t fml_qk_norm_rope_bwd(fml_ctx* ctx, const float* q, int64_t ld_q, const f
   int grid;
   rc = launch<true>(ctx, p, &grid);
   if (rc || !p.parts) return rc;
-  qk_gain_kernel<<<(2 * d_head + 31) / 32, THREADS, 0, ctx->stream>>>(scratch, grid, d_head, dgain_q, dgain_k);
-  FML_LAUNCH_CHECK(ctx, "qk_gain_kernel");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * d_head + 31) / 32);
+  cfg.blockDim = dim3(1024);
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  FML_CUDA(ctx, cudaLaunchKernelEx(&cfg, qk_gain_kernel, (const float*)scratch, grid, (int)d_head, dgain_q, dgain_k));
   return FML_OK;
 }
 
