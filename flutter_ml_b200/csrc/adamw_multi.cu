@@ -82,6 +82,8 @@ __host__ __device__ inline Hyper hyper_at(const HyperIn& p, int t) {
 
 struct DeviceStep { Hyper h; int t; };   // the plan's own step counter, advanced on the device (captured launches included)
 __global__ void advance_kernel(DeviceStep* d, const HyperIn p) {
+  fml_chain_next();
+  fml_chain_wait();
   if (d->t < 0x7fffffff) d->t++;
   d->h = hyper_at(p, d->t);
 }
@@ -298,8 +300,11 @@ __device__ __forceinline__ void update_block(Block<EIGHT>& k, float* mbuf, float
 
 template <bool EIGHT, bool NEAREST, bool ZERO>
 __global__ void __launch_bounds__(32 * WARPS, EIGHT ? 5 : 1) adamw_kernel(const Item* __restrict__ items, float* __restrict__ mbuf, float* __restrict__ vbuf, long long n_blocks, Hyper h, const DeviceStep* __restrict__ dev) {
+  fml_chain_next();
+  const Item it = items[blockIdx.x];                  // the plan's own table: written before any step
+  fml_chain_wait();
   Block<EIGHT> k;
-  load_block(k, items[blockIdx.x], mbuf, vbuf, n_blocks);
+  load_block(k, it, mbuf, vbuf, n_blocks);
   if (dev) h = dev->h;
   update_block<EIGHT, NEAREST, ZERO>(k, mbuf, vbuf, n_blocks, h);
 }
@@ -430,8 +435,7 @@ int32_t fml_adamw_plan_step(fml_ctx* ctx, int32_t plan_id, int32_t lane, double 
   const HyperIn in = {lr, beta1, beta2, eps, weight_decay, grad_scale, seed};
   const DeviceStep* dev = nullptr;
   if (t == 0) {
-    advance_kernel<<<1, 1, 0, s>>>(p->step, in);
-    FML_LAUNCH_CHECK(ctx, "advance_kernel");
+    FML_CUDA(ctx, fml_launch_chained(advance_kernel, dim3(1), dim3(1), 0, s, p->step, in));
     dev = p->step;
   }
   if (p->n_items == 0) return FML_OK;
@@ -440,8 +444,7 @@ int32_t fml_adamw_plan_step(fml_ctx* ctx, int32_t plan_id, int32_t lane, double 
   auto* k = p->bits == 32 ? (zero ? adamw_kernel<false, true, true> : adamw_kernel<false, true, false>)
             : nearest     ? (zero ? adamw_kernel<true, true, true> : adamw_kernel<true, true, false>)
                           : (zero ? adamw_kernel<true, false, true> : adamw_kernel<true, false, false>);
-  k<<<p->n_items, 32 * WARPS, 0, s>>>(p->items, p->m, p->v, p->n_blocks, h, dev);
-  FML_LAUNCH_CHECK(ctx, "adamw_kernel");
+  FML_CUDA(ctx, fml_launch_chained(k, dim3(p->n_items), dim3(32 * WARPS), 0, s, p->items, p->m, p->v, p->n_blocks, h, dev));
   return FML_OK;
 }
 

@@ -100,6 +100,26 @@ int32_t fml_ensure_workspace_keep(fml_ctx* ctx, size_t bytes);
       return fml_fail((ctx), FML_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e__)); \
   } while (0)
 
+// Launches a kernel that may be set up while the kernel before it on the stream drains (programmatic dependent launch).  Such
+// a kernel calls fml_chain_next() at its start, so that the one behind it can do the same, and fml_chain_wait() before it
+// touches global memory: that returns when everything before it has finished and is visible.
+template <class... K, class... A>
+inline cudaError_t fml_launch_chained(void (*kernel)(K...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<K>(args)...);
+}
+__device__ __forceinline__ void fml_chain_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void fml_chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // Second word of the context's status block: set (first writer wins) by a kernel that met a token id or a class label
 // outside its range.  The kernel skips the access, so a bad index is a reported error, never an illegal address.
 #define FML_STATUS_BAD_INDEX_WORD 1

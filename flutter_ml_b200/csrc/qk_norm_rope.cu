@@ -230,7 +230,9 @@ __global__ void __launch_bounds__(THREADS, BWD ? CTAS_BWD : CTAS_FWD) qk_vec_ker
   at.e0 = at.turned ? 4 * at.u : p.rot + 4 * (at.u - (p.rot >> 3));
   at.e1 = at.turned ? 4 * at.u + at.half : at.e0 + ((d - p.rot) >> 1);
   __shared__ double freq[MAX_D / 2];
+  fml_chain_next();
   frequencies(p, freq);
+  fml_chain_wait();
   float* cosv = sm;
   float* sinv = sm + p.rows_cta * at.half;
   float dg[2][8];
@@ -276,7 +278,9 @@ __global__ void __launch_bounds__(THREADS) qk_pair_kernel(const Params p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int half = p.rot >> 1, d = p.d;
   __shared__ double freq[MAX_D / 2];
+  fml_chain_next();
   frequencies(p, freq);
+  fml_chain_wait();
   float* cosv = sm;
   float* sinv = sm + p.rows_cta * half;
   const int total = p.s[0].heads + p.s[1].heads;
@@ -390,7 +394,8 @@ __global__ void __launch_bounds__(THREADS) qk_pair_kernel(const Params p) {
 __global__ void __launch_bounds__(1024) qk_gain_kernel(const float* __restrict__ parts, int n_parts, int d, float* dgain_q, float* dgain_k) {
   __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
-  asm volatile("griddepcontrol.wait;" ::: "memory");   // the launch overlaps the main kernel's end, the reading does not
+  fml_chain_next();
+  fml_chain_wait();
   constexpr int PER = (MAX_PARTS + 31) / 32;
   float v[PER], sum = 0.f;
 #pragma unroll
@@ -469,9 +474,8 @@ bool can_vec(Params& p) {
 }
 
 template <int LPH, bool BWD>
-void launch_vec(const Params& p, int grid, size_t smem, cudaStream_t s) {
-  if (p.interleaved) qk_vec_kernel<LPH, BWD, true><<<grid, THREADS, smem, s>>>(p);
-  else qk_vec_kernel<LPH, BWD, false><<<grid, THREADS, smem, s>>>(p);
+cudaError_t launch_vec(const Params& p, int grid, size_t smem, cudaStream_t s) {
+  return fml_launch_chained(p.interleaved ? qk_vec_kernel<LPH, BWD, true> : qk_vec_kernel<LPH, BWD, false>, dim3(grid), dim3(THREADS), smem, s, p);
 }
 
 template <bool BWD>
@@ -484,12 +488,12 @@ int32_t launch(fml_ctx* ctx, Params& p, int* grid_out) {
   p.rows_cta = (int)std::min<long long>(std::min(32, 8192 / std::max(p.rot, 1)), (p.rows + grid - 1) / grid);
   const int rc = p.rows_cta;
   const size_t smem = std::max<size_t>((size_t)rc * p.rot * 4, BWD ? (size_t)WARPS * 2 * p.d * 4 : 0);   // at most 32 KB
-  if (!vec) qk_pair_kernel<BWD><<<grid, THREADS, smem, ctx->stream>>>(p);
-  else if (lph == 4) launch_vec<4, BWD>(p, grid, smem, ctx->stream);
-  else if (lph == 8) launch_vec<8, BWD>(p, grid, smem, ctx->stream);
-  else if (lph == 16) launch_vec<16, BWD>(p, grid, smem, ctx->stream);
-  else launch_vec<32, BWD>(p, grid, smem, ctx->stream);
-  FML_LAUNCH_CHECK(ctx, "qk_norm_rope kernel");
+  const cudaError_t e = !vec        ? fml_launch_chained(qk_pair_kernel<BWD>, dim3(grid), dim3(THREADS), smem, ctx->stream, p)
+                        : lph == 4  ? launch_vec<4, BWD>(p, grid, smem, ctx->stream)
+                        : lph == 8  ? launch_vec<8, BWD>(p, grid, smem, ctx->stream)
+                        : lph == 16 ? launch_vec<16, BWD>(p, grid, smem, ctx->stream)
+                                    : launch_vec<32, BWD>(p, grid, smem, ctx->stream);
+  if (e != cudaSuccess) return fml_fail(ctx, FML_ERR_CUDA, std::string("qk_norm_rope kernel: ") + cudaGetErrorString(e));
   *grid_out = grid;
   return FML_OK;
 }
@@ -538,16 +542,7 @@ int32_t fml_qk_norm_rope_bwd(fml_ctx* ctx, const float* q, int64_t ld_q, const f
   int grid;
   rc = launch<true>(ctx, p, &grid);
   if (rc || !p.parts) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(2 * d_head + 31) / 32);
-  cfg.blockDim = dim3(1024);
-  cfg.stream = ctx->stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  FML_CUDA(ctx, cudaLaunchKernelEx(&cfg, qk_gain_kernel, (const float*)scratch, grid, (int)d_head, dgain_q, dgain_k));
+  FML_CUDA(ctx, fml_launch_chained(qk_gain_kernel, dim3((unsigned)(2 * d_head + 31) / 32), dim3(1024), 0, ctx->stream, scratch, grid, d_head, dgain_q, dgain_k));
   return FML_OK;
 }
 

@@ -158,6 +158,8 @@ __global__ void __launch_bounds__(32 * WARPS) scan_kernel(const Params p) {
   const int unit = blockIdx.x / cs;
   const int seq = unit / p.ctiles, c = (unit - seq * p.ctiles) * CW + ch;
   const bool on = c < p.dim;
+  fml_chain_next();
+  fml_chain_wait();
   const int len = length_of(p, seq);
   const float* f = p.f + seq * p.ss_in + c;
   const float* x = p.x + seq * p.ss_in + c;
@@ -328,6 +330,8 @@ __global__ void __launch_bounds__(32 * WARPS) scan_kernel(const Params p) {
 template <bool GATED, bool BWD>
 __global__ void __launch_bounds__(THREADS) step_kernel(const Params p) {
   const long long i = blockIdx.x * (long long)THREADS + threadIdx.x;
+  fml_chain_next();
+  fml_chain_wait();
   if (i >= (long long)p.n_seq * p.dim) return;
   const int seq = (int)(i / p.dim), c = (int)(i - (long long)seq * p.dim);
   const int len = length_of(p, seq);
@@ -414,10 +418,15 @@ int32_t launch_scan(fml_ctx* ctx, Params& p, int cluster) {
   cfg.blockDim = dim3(32 * WARPS);
   cfg.stream = ctx->stream;
   cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim = {(unsigned)cluster, 1, 1};
+  if (TEAM) {
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim = {(unsigned)cluster, 1, 1};
+  } else {   // set up while the kernel before drains; with clusters that was slower (203 us against 165 on the long sequence)
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+  }
   cfg.attrs = at;
-  cfg.numAttrs = TEAM ? 1 : 0;
+  cfg.numAttrs = 1;
   FML_CUDA(ctx, cudaLaunchKernelEx(&cfg, scan_kernel<WARPS, LANES, VEC, SEG, GATED, BWD, AHEAD, TEAM>, (const Params)p));
   return FML_OK;
 }
@@ -435,15 +444,20 @@ int32_t launch_lanes(fml_ctx* ctx, Params& p) {
   constexpr int SEG = 16 / VEC;
   auto units = [&](int lanes) { return (long long)p.n_seq * ((p.dim + lanes * VEC - 1) / (lanes * VEC)); };
   const int sms = ctx->sm_count;
-  // Channels enough: CTAs of four warps, each over all steps of its channels, rows as wide as leaves four CTAs an SM
+  // Channels enough: each CTA goes over all steps of its channels, the next round's rows in registers meanwhile; rows of 32
+  // lanes where that leaves three CTAs of four warps an SM, else of 16 or 8 (128 sequences of 128 x 512: 21.2 us forward and
+  // 38 backward with 32 lanes, 21.6 and 40 with 16; 32 ragged ones of 512 x 1024: 23.4 and 40.6 with 8, 25.6 and 40.7 with 16),
+  // CTAs of eight warps where there are few (8 of 2048 x 1024: 36 and 70; four warps 46 and 70, clusters 57 and 118).
   if (units(32) >= 3 * sms) return launch_scan<4, 32, VEC, SEG, GATED, BWD, true, false>(ctx, p, 1);
   if (units(16) >= 4 * sms) return launch_scan<4, 16, VEC, SEG, GATED, BWD, true, false>(ctx, p, 1);
   if (units(8) >= 4 * sms) return launch_scan<4, 8, VEC, SEG, GATED, BWD, true, false>(ctx, p, 1);
   if (units(8) >= sms) return launch_scan<8, 8, VEC, SEG, GATED, BWD, true, false>(ctx, p, 1);
-  // Few: eight warps, narrow rows, and a cluster along the steps until there are two CTAs an SM
+  // Few: eight warps, rows of four lanes, long segments forward, and a cluster along the steps that gives two CTAs an SM (one
+  // sequence of 65521 x 250: 62 and 105 us with eight CTAs, 75 and 118 with four; with the next round in registers there is
+  // one CTA an SM, 68 and 127).
   constexpr int LONG = BWD ? SEG : 2 * SEG;
-  int cluster = 1;
-  while (cluster < MAX_CLUSTER && units(4) * cluster * 2 <= 2 * sms && 64ll * LONG * cluster < p.seq_len) cluster <<= 1;
+  int cluster = (int)std::min<long long>(MAX_CLUSTER, 2 * sms / units(4));
+  while (cluster > 1 && 64ll * LONG * (cluster - 1) >= p.seq_len) cluster--;   // every CTA has steps
   if (cluster > 1) return launch_scan<8, 4, VEC, LONG, GATED, BWD, false, true>(ctx, p, cluster);
   return launch_scan<8, 4, VEC, LONG, GATED, BWD, false, false>(ctx, p, 1);
 }
@@ -452,9 +466,9 @@ template <bool GATED, bool BWD>
 int32_t launch(fml_ctx* ctx, Params& p) {
   if (p.n_seq == 0) return FML_OK;
   if (p.seq_len <= 4) {
-    step_kernel<GATED, BWD><<<(unsigned)(((long long)p.n_seq * p.dim + THREADS - 1) / THREADS), THREADS, 0, ctx->stream>>>(p);
-    FML_LAUNCH_CHECK(ctx, "step_kernel");
-    return FML_OK;
+    const unsigned blocks = (unsigned)(((long long)p.n_seq * p.dim + THREADS - 1) / THREADS);
+    const cudaError_t e = fml_launch_chained(step_kernel<GATED, BWD>, dim3(blocks), dim3(THREADS), 0, ctx->stream, p);
+    return e == cudaSuccess ? FML_OK : fml_fail(ctx, FML_ERR_CUDA, std::string("step_kernel: ") + cudaGetErrorString(e));
   }
   const int vec = vector_width(p);
   if (vec == 4) return launch_lanes<4, GATED, BWD>(ctx, p);
