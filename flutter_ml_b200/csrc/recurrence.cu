@@ -30,6 +30,7 @@ namespace {
 
 constexpr int THREADS = 256;
 constexpr int MAX_CLUSTER = 8;
+constexpr int WAIT_CODE = 130;   // fml_device_status: a cluster's pairs did not arrive
 
 struct Params {
   const float *f, *x, *h0, *h, *dy, *dh_last;
@@ -65,10 +66,39 @@ __device__ __forceinline__ void gate(float f, float& a, float& s) {
 template <bool GATED>
 __device__ __forceinline__ float through(float A, float B, float state) { return !GATED && state == 0.f ? B : fmaf(A, state, B); }
 
-__device__ __forceinline__ void store_remote(const float* here, uint32_t rank, float v) {
-  uint32_t there;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(fml_tc::smem_u32(here)), "r"(rank));
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(v) : "memory");
+// A pair into the shared memory of CTA `rank` of the cluster, counted by that CTA's barrier: neither side needs a fence, which
+// would wait for the results of the round before as well (the cluster's own barrier did).
+__device__ __forceinline__ void send_pair(const float2* here, const uint64_t* bar, uint32_t rank, float2 v) {
+  uint32_t to, sig;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(fml_tc::smem_u32(here)), "r"(rank));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(sig) : "r"(fml_tc::smem_u32(bar)), "r"(rank));
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(to), "f"(v.x), "f"(v.y), "r"(sig)
+               : "memory");
+}
+
+// Waits for a set's bytes, WAIT_LIMIT_NS at most: then the status word gets a code, the CTA waits for nothing more, and the
+// results are whatever they are.
+__device__ __forceinline__ void wait_pairs(uint32_t bar, uint32_t parity, volatile int* gave_up, int* status) {
+  unsigned long long t0 = 0;
+  for (uint32_t spins = 0;; spins++) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return;
+    if (spins == 0) t0 = fml_tc::globaltimer_ns();
+    if ((spins & 0xFF) != 0xFF) continue;
+    if (*gave_up) return;
+    if (fml_tc::globaltimer_ns() - t0 > fml_tc::WAIT_LIMIT_NS) {
+      *gave_up = 1;
+      atomicCAS(status, 0, WAIT_CODE);
+      return;
+    }
+  }
 }
 
 __device__ __forceinline__ int length_of(const Params& p, int seq) {
@@ -90,6 +120,10 @@ __device__ __forceinline__ void store_row(float* dst, const float* src) {
   else if (VEC == 2) *reinterpret_cast<float2*>(dst) = *reinterpret_cast<const float2*>(src);
   else *dst = *src;
 }
+
+// CTAs an SM that a scan is compiled for.  Forward 128 registers a thread (128 sequences of 128 x 512: 18.5 us; left alone the
+// compiler takes 200 and it is 23).  Backward the next round's four rows need them: 35 us with any number, 47 with 128.
+constexpr int min_ctas(int warps, bool team, bool bwd) { return team ? 2 : bwd ? 1 : 16 / warps; }
 
 // What a lane has read of its segment, SEG steps of VEC channels, in scan direction.
 template <int VEC, int SEG, bool BWD>
@@ -146,12 +180,16 @@ __device__ __forceinline__ void load_segment(const Params& p, Raw<VEC, SEG, BWD>
 }
 
 template <int WARPS, int LANES, int VEC, int SEG, bool GATED, bool BWD, bool AHEAD, bool TEAM>
-__global__ void __launch_bounds__(32 * WARPS) scan_kernel(const Params p) {
+__global__ void __launch_bounds__(32 * WARPS, min_ctas(WARPS, TEAM, BWD)) scan_kernel(const Params p) {
   constexpr int SUBS = 32 / LANES;                    // segments of a warp that share their channels
   constexpr int CW = LANES * VEC;                     // channels of a CTA
   constexpr int TILE = WARPS * SUBS * SEG;            // steps of a CTA's round
   __shared__ __align__(16) float wtot[2][WARPS][2][CW];   // the warps' pairs; two sets, so one barrier a round is enough
-  __shared__ __align__(16) float ctot[TEAM ? 2 : 1][TEAM ? MAX_CLUSTER : 1][2][CW];   // the CTAs' pairs, written by their owners into every CTA
+  // The CTAs' pairs, written by their owners into every CTA.  Two sets: a CTA sends round r + 2's pairs when it has every
+  // CTA's of round r + 1, and those were sent when their owners had read round r's.
+  __shared__ __align__(16) float2 ctot[TEAM ? 2 : 1][TEAM ? MAX_CLUSTER : 1][CW];
+  __shared__ uint64_t arrived[2];                     // counts the bytes of a set
+  __shared__ int gave_up;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int ch = (lane % LANES) * VEC, sub = lane / LANES;
   const int cs = TEAM ? p.cluster : 1, rank = TEAM ? (int)fml_tc::cluster_ctarank() : 0;
@@ -173,9 +211,17 @@ __global__ void __launch_bounds__(32 * WARPS) scan_kernel(const Params p) {
     state[v] = !BWD ? first[v] : on && p.dh_last ? p.dh_last[edge + v] : 0.f;
   }
   Raw<VEC, SEG, BWD> raw;
-  if (TEAM) fml_tc::cluster_sync_all();               // every CTA is there before the first remote store
+  if (TEAM) {
+    if (threadIdx.x == 0) {
+      gave_up = 0;
+      for (int i = 0; i < 2; i++) fml_tc::mbar_init(fml_tc::smem_u32(&arrived[i]), 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    fml_tc::cluster_sync_all();                       // every CTA's barriers are there, and every CTA has read h0 and dh_last
+  }
   int p0 = ((rank * WARPS + warp) * SUBS + sub) * SEG;   // first step of the segment, counted in scan direction
   if (AHEAD) load_segment<VEC, SEG, GATED, BWD>(p, raw, f, x, h, dy, first, p0, len, on);
+  uint32_t phase = 0;
   for (int base = 0, buf = 0; base < len; base += TILE * cs, p0 += TILE * cs, buf ^= 1) {
     if (!AHEAD) load_segment<VEC, SEG, GATED, BWD>(p, raw, f, x, h, dy, first, p0, len, on);
     // forward: decay and input; backward: decay, incoming gradient, and what G is multiplied by for dx and df
@@ -230,7 +276,8 @@ __global__ void __launch_bounds__(32 * WARPS) scan_kernel(const Params p) {
     __syncthreads();
     float run[VEC];                                   // the state before the lane's steps; `state`: after the round
     if (TEAM) {
-      // the CTA's pair into every CTA of the cluster; two sets of places, so one cluster barrier a round is enough
+      const uint32_t bar = fml_tc::smem_u32(&arrived[buf]);
+      if (threadIdx.x == 0) fml_tc::mbar_expect_tx(bar, (uint32_t)(cs * CW * sizeof(float2)));
       for (int i = threadIdx.x; i < cs * CW; i += 32 * WARPS) {
         const int r = i / CW, k = i - r * CW;
         float At = 1.f, Bt = 0.f;
@@ -240,21 +287,17 @@ __global__ void __launch_bounds__(32 * WARPS) scan_kernel(const Params p) {
           Bt = through<GATED>(Aq, wtot[buf][q][1][k], Bt);
           At *= Aq;
         }
-        store_remote(&ctot[buf][rank][0][k], r, At);
-        store_remote(&ctot[buf][rank][1][k], r, Bt);
+        send_pair(&ctot[buf][rank][k], &arrived[buf], r, make_float2(At, Bt));
       }
-      __syncwarp();
-      fml_tc::cluster_sync_all();
-      for (int r = 0; r < cs; r++) {
-        float Ar[VEC], Br[VEC];
-        load_row<VEC>(Ar, &ctot[buf][r][0][ch]);
-        load_row<VEC>(Br, &ctot[buf][r][1][ch]);
+      wait_pairs(bar, phase, &gave_up, p.status);
+      phase ^= buf;                                   // each set is used every other round
+      for (int r = 0; r < cs; r++)
 #pragma unroll
         for (int v = 0; v < VEC; v++) {
+          const float2 pr = ctot[buf][r][ch + v];
           if (r == rank) run[v] = state[v];
-          state[v] = through<GATED>(Ar[v], Br[v], state[v]);
+          state[v] = through<GATED>(pr.x, pr.y, state[v]);
         }
-      }
 #pragma unroll
       for (int q = 0; q < WARPS - 1; q++)
         if (q < warp) {
@@ -319,6 +362,7 @@ __global__ void __launch_bounds__(32 * WARPS) scan_kernel(const Params p) {
       }
     }
   }
+  if (TEAM) fml_tc::cluster_sync_all();               // nobody leaves while something may still arrive
   float* last = BWD ? p.dh0 : p.last;
   if (last && on && rank == 0 && warp == 0 && sub == 0) {
 #pragma unroll
@@ -445,16 +489,17 @@ int32_t launch_lanes(fml_ctx* ctx, Params& p) {
   auto units = [&](int lanes) { return (long long)p.n_seq * ((p.dim + lanes * VEC - 1) / (lanes * VEC)); };
   const int sms = ctx->sm_count;
   // Channels enough: each CTA goes over all steps of its channels, the next round's rows in registers meanwhile; rows of 32
-  // lanes where that leaves three CTAs of four warps an SM, else of 16 or 8 (128 sequences of 128 x 512: 21.2 us forward and
-  // 38 backward with 32 lanes, 21.6 and 40 with 16; 32 ragged ones of 512 x 1024: 23.4 and 40.6 with 8, 25.6 and 40.7 with 16),
+  // lanes where that leaves three CTAs of four warps an SM, else of 16 or 8 (before the last steps, 128 sequences of 128 x 512:
+  // 21.2 us forward and 38 backward with 32 lanes, 21.6 and 40 with 16; 32 ragged ones of 512 x 1024: 23.4 and 40.6 with 8, 25.6
+  // and 40.7 with 16),
   // CTAs of eight warps where there are few (8 of 2048 x 1024: 36 and 70; four warps 46 and 70, clusters 57 and 118).
   if (units(32) >= 3 * sms) return launch_scan<4, 32, VEC, SEG, GATED, BWD, true, false>(ctx, p, 1);
   if (units(16) >= 4 * sms) return launch_scan<4, 16, VEC, SEG, GATED, BWD, true, false>(ctx, p, 1);
   if (units(8) >= 4 * sms) return launch_scan<4, 8, VEC, SEG, GATED, BWD, true, false>(ctx, p, 1);
   if (units(8) >= sms) return launch_scan<8, 8, VEC, SEG, GATED, BWD, true, false>(ctx, p, 1);
   // Few: eight warps, rows of four lanes, long segments forward, and a cluster along the steps that gives two CTAs an SM (one
-  // sequence of 65521 x 250: 62 and 105 us with eight CTAs, 75 and 118 with four; with the next round in registers there is
-  // one CTA an SM, 68 and 127).
+  // sequence of 65521 x 250: 61 and 97 us with eight CTAs; rows of eight lanes, half the CTAs, 91 and 135; one of 16384 x 1024:
+  // 44 and 78 with four).
   constexpr int LONG = BWD ? SEG : 2 * SEG;
   int cluster = (int)std::min<long long>(MAX_CLUSTER, 2 * sms / units(4));
   while (cluster > 1 && 64ll * LONG * (cluster - 1) >= p.seq_len) cluster--;   // every CTA has steps
