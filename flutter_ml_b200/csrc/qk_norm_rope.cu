@@ -47,7 +47,8 @@ struct Params {
   Side s[2];
   const int* pos;
   float* parts;        // [CTA][2][d], or NULL when no gain gradient is wanted
-  long long rows;
+  long long rows, each;  // each: rows of a CTA, one more in the first `more` CTAs
+  int more;
   int seq_len, d, rot, interleaved, accumulate;
   int rows_cta;        // rows whose angles a CTA forms at once
   double kexp;         // -2 log2(base) / rot
@@ -61,10 +62,11 @@ __device__ __forceinline__ void frequencies(const Params& p, double* freq) {
 // cosines and sines of rows [r0, r0 + n), rot / 2 each a row
 __device__ __forceinline__ void angles(const Params& p, const double* freq, long long r0, int n, float* cosv, float* sinv) {
   const int half = p.rot >> 1;
+  const long long first = p.seq_len > 0 ? r0 % p.seq_len : r0;
   for (int i = threadIdx.x; i < n * half; i += THREADS) {
-    const int r = i / half, j = i - r * half;
-    const long long row = r0 + r;
-    const double turns = (p.pos ? (double)p.pos[row] : (double)(p.seq_len > 0 ? row % p.seq_len : row)) * freq[j];
+    const int r = (int)((unsigned)i / (unsigned)half), j = i - r * half;
+    const double pos = p.pos ? (double)p.pos[r0 + r] : p.seq_len > 0 ? (double)((unsigned)(first + r) % (unsigned)p.seq_len) : (double)(first + r);
+    const double turns = pos * freq[j];
     float s, c;
     sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
     cosv[i] = c;
@@ -73,10 +75,7 @@ __device__ __forceinline__ void angles(const Params& p, const double* freq, long
 }
 
 // first row of CTA b's share: neighbouring rows, the shares equal to a row
-__device__ __forceinline__ long long share(long long rows, unsigned b) {
-  const long long each = rows / gridDim.x, more = rows - each * gridDim.x;
-  return each * b + min((long long)b, more);
-}
+__device__ __forceinline__ long long share(const Params& p, unsigned b) { return p.each * b + min(b, (unsigned)p.more); }
 
 template <int LPH>
 __device__ __forceinline__ float head_sum(float v) {
@@ -240,8 +239,8 @@ __global__ void __launch_bounds__(THREADS, BWD ? CTAS_BWD : CTAS_FWD) qk_vec_ker
   for (int t = 0; t < 2; t++)
 #pragma unroll
     for (int i = 0; i < 8; i++) dg[t][i] = 0.f;
-  const long long last = share(p.rows, blockIdx.x + 1);
-  for (long long r0 = share(p.rows, blockIdx.x); r0 < last; r0 += p.rows_cta) {
+  const long long last = share(p, blockIdx.x + 1);
+  for (long long r0 = share(p, blockIdx.x); r0 < last; r0 += p.rows_cta) {
     const int n = (int)min((long long)p.rows_cta, last - r0);
     __syncthreads();                                  // the table of the step before has been read
     angles(p, freq, r0, n, cosv, sinv);
@@ -300,8 +299,8 @@ __global__ void __launch_bounds__(THREADS) qk_pair_kernel(const Params p) {
     dg[0][j][0] = dg[0][j][1] = dg[1][j][0] = dg[1][j][1] = 0.f;
   }
   const float inv_d = 1.f / (float)d;
-  const long long last = share(p.rows, blockIdx.x + 1);
-  for (long long r0 = share(p.rows, blockIdx.x); r0 < last; r0 += p.rows_cta) {
+  const long long last = share(p, blockIdx.x + 1);
+  for (long long r0 = share(p, blockIdx.x); r0 < last; r0 += p.rows_cta) {
     const int n = (int)min((long long)p.rows_cta, last - r0);
     __syncthreads();
     angles(p, freq, r0, n, cosv, sinv);
@@ -485,6 +484,8 @@ int32_t launch(fml_ctx* ctx, Params& p, int* grid_out) {
   const int fit = ctx->sm_count * (BWD ? CTAS_BWD : CTAS_FWD);
   const int grid = (int)std::min<long long>({p.rows, fit, BWD ? MAX_PARTS : fit});
   // rows whose angles are formed at once: a table of 32 KB at most, and no more than the CTA has
+  p.each = p.rows / grid;
+  p.more = (int)(p.rows % grid);
   p.rows_cta = (int)std::min<long long>(std::min(32, 8192 / std::max(p.rot, 1)), (p.rows + grid - 1) / grid);
   const int rc = p.rows_cta;
   const size_t smem = std::max<size_t>((size_t)rc * p.rot * 4, BWD ? (size_t)WARPS * 2 * p.d * 4 : 0);   // at most 32 KB

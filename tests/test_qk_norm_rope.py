@@ -147,6 +147,11 @@ CASES = [
     dict(rows=31, hq=2, hk=2, d=256, rot=0),
     dict(rows=20000, hq=2, hk=1, d=64, rot=64, positions=512),                    # more rows than one round of CTAs takes
     dict(rows=3001, hq=1, hk=1, d=10, rot=6),
+    dict(rows=77, hq=5, hk=2, d=24, rot=8),                                       # three lanes a head, ten heads a warp
+    dict(rows=201, hq=7, hk=7, d=40, rot=40, shift=2),
+    dict(rows=45, hq=9, hk=3, d=72, rot=64, interleaved=True),
+    dict(rows=700, hq=1, hk=1, d=16, rot=0),
+    dict(rows=4999, hq=12, hk=3, d=80, rot=32, interleaved=True, pad=7),
 ]
 
 
