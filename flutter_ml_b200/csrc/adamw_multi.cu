@@ -103,29 +103,48 @@ __device__ __forceinline__ void decode8(uint32_t codes, float* out) {
 // exponent of the block's scale from the bits of its largest finite absolute value
 __device__ __forceinline__ int scale_exponent(uint32_t amax) { return max((int)((amax + 0x1FFFFFu) >> 23) - 135, -126); }
 
-// What brings x down to x / scale * 2^-120: then 2^-6, the format's smallest normal number, is float's smallest normal number,
-// and the float's bits from the twentieth on ARE the code, subnormal or not, and those below are what is rounded away.
-// Scales above 2^29 need the power in two parts (`pre` is 1 otherwise).
-struct Down {
-  float pre, by;
-};
-__device__ __forceinline__ Down down(int e) {
-  const int pre = e > 29 ? 120 : 0, rest = -120 - e + pre;   // -149 <= rest <= 6
-  return {pre ? 0x1p-120f : 1.f, rest >= -126 ? __int_as_float((rest + 127) << 23) : __int_as_float(1 << (rest + 149))};
+// Scales whose power of two, brought down by 2^-120, is still a float: larger ones take the rare way (see encode8)
+constexpr int BIG_SCALE = 29;
+__device__ __forceinline__ float power_of_two(int e) {   // -149 .. 127
+  return e >= -126 ? __int_as_float((e + 127) << 23) : __int_as_float(1 << (e + 149));
 }
-// those bits with the rounding added, the sign on top
-template <bool NEAREST>
-__device__ __forceinline__ uint32_t encode8(float x, const Down& d, uint32_t rnd16) {
-  const uint32_t z = __float_as_uint(__fmul_rn(d.pre != 1.f ? __fmul_rn(x, d.pre) : x, d.by));
-  return z + (NEAREST ? 0x7FFFFu + ((z >> 20) & 1u) : rnd16 * 16u);
+
+// `down` brings x to x / scale * 2^-120: then 2^-6, the format's smallest normal number, is float's smallest normal number, and
+// the float's bits from the twentieth on ARE the code, subnormal or not, and those below are what is rounded away.  Returns
+// them with the rounding added, moved up by four: the code in the upper byte.  `up16` is the random number in bits 8 .. 23.
+template <bool NEAREST, bool SIGNED>
+__device__ __forceinline__ uint32_t encode8(float x, float down, uint32_t up16) {
+  const uint32_t z = __float_as_uint(__fmul_rn(x, down));
+  const uint32_t t = NEAREST ? (z + 0x7FFFFu + ((z >> 20) & 1u)) * 16u : z * 16u + up16;
+  return SIGNED ? t | (z & 0x80000000u) : t;
 }
-// the codes of four encoded numbers
-template <bool SIGNED>
+// the upper bytes of four numbers
 __device__ __forceinline__ uint32_t pack8(const uint32_t* z) {
-  uint32_t b[4];
+  return __byte_perm(__byte_perm(z[0], z[1], 0x0073), __byte_perm(z[2], z[3], 0x0073), 0x5410);
+}
+
+// Square roots of eight numbers >= 0, one Newton step on the hardware's reciprocal root (Markstein's form: the residual
+// v - s s is exact, so the result is the rounded root but for about one number in a million, one unit off).  Zeros, the
+// smallest numbers and what is not finite go through the library's root: half of it is the test for them, here made once.
+__device__ __forceinline__ void roots8(const float* v, float* root) {
+  float least = INFINITY, all = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; i++) b[i] = SIGNED ? z[i] << 4 | (z[i] & 0x80000000u) : z[i] << 4;
-  return __byte_perm(__byte_perm(b[0], b[1], 0x0073), __byte_perm(b[2], b[3], 0x0073), 0x5410);
+  for (int j = 0; j < 8; j++) {
+    least = fminf(least, v[j]);
+    all += v[j];
+  }
+  if (least >= 0x1p-100f && all < INFINITY) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      float y;
+      asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(v[j]));
+      const float s = v[j] * y;
+      root[j] = fmaf(fmaf(-s, s, v[j]), 0.5f * y, s);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; j++) root[j] = __fsqrt_rn(v[j]);
+  }
 }
 
 // A warp's block on its way through the registers: eight elements a lane, 4 l .. 4 l + 3 and 128 + 4 l ..
@@ -195,7 +214,10 @@ __device__ __forceinline__ void update_block(Block<EIGHT>& k, float* mbuf, float
   }
   float* mv = EIGHT ? m8 : k.mv;
   float* vv = EIGHT ? v8 : k.vv;
-  float root[8], mmax = 0.f, rmax = 0.f, all = 0.f;
+  if (h.gs != 1.f) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) k.gv[j] = __fmul_rn(k.gv[j], h.gs);
+  }
 #pragma unroll
   for (int j = 0; j < 8; j++) {
     float m = mv[j], v = vv[j];
@@ -204,17 +226,20 @@ __device__ __forceinline__ void update_block(Block<EIGHT>& k, float* mbuf, float
       v = __fmul_rn(v, k.rs);
       v = __fmul_rn(v, v);
     }
-    const float gj = __fmul_rn(k.gv[j], h.gs);
-    m = __fadd_rn(__fmul_rn(m, h.b1), __fmul_rn(gj, h.omb1));
-    v = __fadd_rn(__fmul_rn(v, h.b2), __fmul_rn(__fmul_rn(gj, gj), h.omb2));
-    root[j] = __fsqrt_rn(v);
+    const float gj = k.gv[j];
+    mv[j] = __fadd_rn(__fmul_rn(m, h.b1), __fmul_rn(gj, h.omb1));
+    vv[j] = __fadd_rn(__fmul_rn(v, h.b2), __fmul_rn(__fmul_rn(gj, gj), h.omb2));
+  }
+  float root[8], mmax = 0.f, rmax = 0.f, all = 0.f;
+  roots8(vv, root);
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const float m = mv[j];
     // the hardware's reciprocal, good to one unit in the last place: it moves w by lr times that
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(fmaf(root[j], h.rc2, h.eps)));
     k.wv[j] -= h.step * m * inv;
     k.wv[j] -= h.decay * k.wv[j];
-    mv[j] = m;
-    vv[j] = v;
     if (EIGHT) {
       mmax = fmaxf(mmax, fabsf(m));
       rmax = fmaxf(rmax, root[j]);
@@ -257,7 +282,14 @@ __device__ __forceinline__ void update_block(Block<EIGHT>& k, float* mbuf, float
   }
   const int me = scale_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(mmax)));
   const int re = scale_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(rmax)));
-  const Down md = down(me), rd = down(re);
+  // the rare way of scales above 2^29: the numbers brought down first (those that this takes below float's range have a code of 0)
+  if (me > BIG_SCALE)
+#pragma unroll
+    for (int j = 0; j < 8; j++) mv[j] = finite_bits(__float_as_uint(mv[j])) ? mv[j] * 0x1p-120f : mv[j];
+  if (re > BIG_SCALE)
+#pragma unroll
+    for (int j = 0; j < 8; j++) root[j] = finite_bits(__float_as_uint(root[j])) ? root[j] * 0x1p-120f : root[j];
+  const float md = power_of_two(me > BIG_SCALE ? -me : -120 - me), rd = power_of_two(re > BIG_SCALE ? -re : -120 - re);
   const uint32_t key = NEAREST ? 0u : mix32(h.key + (uint32_t)k.b * 0x9E3779B1u) + 4 * lane;
   uint32_t mo[2], ro[2];
 #pragma unroll
@@ -266,15 +298,15 @@ __device__ __forceinline__ void update_block(Block<EIGHT>& k, float* mbuf, float
 #pragma unroll
     for (int i = 0; i < 4; i++) {
       const uint32_t word = NEAREST ? 0u : mix32(key + (q * 128 + i));
-      zm[i] = encode8<NEAREST>(mv[4 * q + i], md, word >> 16);
-      zr[i] = encode8<NEAREST>(root[4 * q + i], rd, word & 0xffffu);
+      zm[i] = encode8<NEAREST, true>(mv[4 * q + i], md, __byte_perm(word, 0, 0x4324));    // the upper half
+      zr[i] = encode8<NEAREST, false>(root[4 * q + i], rd, __byte_perm(word, 0, 0x4104));  // the lower half
     }
-    mo[q] = pack8<true>(zm);
-    ro[q] = pack8<false>(zr);
+    mo[q] = pack8(zm);
+    ro[q] = pack8(zr);
     if ((ro[q] - 0x01010101u) & 0x80808080u) {        // some code is 0: a positive root keeps the smallest one
 #pragma unroll
       for (int i = 0; i < 4; i++)
-        if ((ro[q] >> (8 * i) & 0xffu) == 0 && root[4 * q + i] > 0.f) ro[q] |= 1u << (8 * i);
+        if ((ro[q] >> (8 * i) & 0xffu) == 0 && vv[4 * q + i] > 0.f) ro[q] |= 1u << (8 * i);
     }
     if (odd) {
 #pragma unroll

@@ -305,6 +305,30 @@ def test_values_that_are_not_finite_stay_in_their_places(ctx):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("seed", [-1, 7])
+def test_blocks_of_extreme_size_bit_for_bit(ctx, seed):
+    """Blocks around 1e15 (scales above 2^29), 1e-15 and 1e-30 (subnormal products), values of 40 orders of magnitude in one."""
+    s = Setup(ctx, [2048], 8, seed=9)
+    rng = np.random.default_rng(9)
+    g = rng.standard_normal(2048).astype(f32)
+    for i, size in enumerate((1e15, 1e17, 1e-15, 1e-18, 1e-30, 1.0, 1e9)):
+        g[256 * i:256 * (i + 1)] *= f32(size)
+    g[1792:] *= np.exp(rng.uniform(-46, 40, 256)).astype(f32)
+    ctx.upload(g, out=s.dg.view(s.off[0], (2048,)))
+    m, r = np.zeros((8, 256), f32), np.zeros((8, 256), f32)
+    for t in (1, 2, 3):
+        s.step(t, seed=seed)
+        (mc, ms), (rc, rs) = s.states(s.m)[0], s.states(s.v)[0]
+        with np.errstate(over="ignore"):
+            m1, v1 = moments32(m, (r * r).astype(f32), padded(g), 0.9, 0.999)
+        rnd = words(8, seed, t) if seed >= 0 else None
+        for got, sc, x, half, root in ((mc, ms, m1, 16, False), (rc, rs, np.sqrt(v1), 0, True)):
+            code, scale = to_codes(x, None if rnd is None else (rnd >> half) & 0xFFFF, root)
+            assert np.array_equal(got, code) and np.array_equal(sc, scale)
+        m, r = to_values(mc, ms), to_values(rc, rs)
+
+
+@pytest.mark.gpu
 def test_small_roots_are_never_rounded_to_zero(ctx):
     """One gradient a million times its neighbours': the neighbours' m and root fall below the block's range, and the root
     stays at 2^-9 of the scale, so a later step with no gradient is bounded by |m| over that."""
