@@ -423,7 +423,7 @@ bool clash(const float* a, long long lda, long long wa, const float* b, long lon
   if (!a || !b || rows == 0 || wa == 0 || wb == 0) return false;
   const uintptr_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
   if (pa + 4 * ((rows - 1) * lda + wa) <= pb || pb + 4 * ((rows - 1) * ldb + wb) <= pa) return false;
-  if (lda != ldb || (pa & 3) != (pb & 3)) return true;
+  if (rows == 1 || lda != ldb || (pa & 3) != (pb & 3)) return true;
   const long long off = ((long long)(pb - pa) / 4 % lda + lda) % lda;   // b's first column, counted from a's
   return off < wa || off + wb > lda;
 }
@@ -466,7 +466,7 @@ int32_t check(fml_ctx* ctx, const Params& p, double base) {
 bool can_vec(Params& p) {
   if (p.d % 8 || p.rot % 8) return false;   // the rest of the head is a multiple of 8 then too
   for (Side& s : p.s) {
-    s.per_head = s.heads > 1 ? (uint32_t)(((1ull << 32) + s.heads - 1) / s.heads) : 0;   // exact below 2^32 / heads
+    s.per_head = s.heads > 1 ? (uint32_t)(((1ull << 32) + s.heads - 1) / s.heads) : 0;   // exact for numbers below 2^32 / heads
     s.wide = (al16(s.x) && s.ldx % 4 == 0 ? 1 : 0) | (al16(s.dy) && s.ldy % 4 == 0 ? 2 : 0) | (al16(s.out) && s.ldo % 4 == 0 ? 4 : 0);
   }
   return true;
@@ -483,10 +483,12 @@ int32_t launch(fml_ctx* ctx, Params& p, int* grid_out) {
   const int lph = p.d <= 32 ? 4 : p.d <= 64 ? 8 : p.d <= 128 ? 16 : 32;
   const int fit = ctx->sm_count * (BWD ? CTAS_BWD : CTAS_FWD);
   const int grid = (int)std::min<long long>({p.rows, fit, BWD ? MAX_PARTS : fit});
-  // rows whose angles are formed at once: a table of 32 KB at most, and no more than the CTA has
   p.each = p.rows / grid;
   p.more = (int)(p.rows % grid);
-  p.rows_cta = (int)std::min<long long>(std::min(32, 8192 / std::max(p.rot, 1)), (p.rows + grid - 1) / grid);
+  // rows whose angles are formed at once: a table of 32 KB at most, no more than the CTA has, and the heads of all of them
+  // times the heads of one below 2^32, where dividing by multiplying is exact
+  const long long heads = std::max(p.s[0].heads, p.s[1].heads);
+  p.rows_cta = (int)std::min<long long>({32, 8192 / std::max(p.rot, 1), (p.rows + grid - 1) / grid, std::max(1ll, (1ll << 31) / (heads * heads))});
   const int rc = p.rows_cta;
   const size_t smem = std::max<size_t>((size_t)rc * p.rot * 4, BWD ? (size_t)WARPS * 2 * p.d * 4 : 0);   // at most 32 KB
   const cudaError_t e = !vec        ? fml_launch_chained(qk_pair_kernel<BWD>, dim3(grid), dim3(THREADS), smem, ctx->stream, p)
@@ -537,6 +539,10 @@ int32_t fml_qk_norm_rope_bwd(fml_ctx* ctx, const float* q, int64_t ld_q, const f
   FML_REQUIRE(ctx, dq_out && (heads_k == 0 || dk_out), "fml_qk_norm_rope_bwd: missing gradient");
   FML_REQUIRE(ctx, (!dgain_q || gain_q) && (!dgain_k || (gain_k && heads_k)), "fml_qk_norm_rope_bwd: the gradient of a gain that is not there");
   FML_REQUIRE(ctx, !(dgain_q || dgain_k) || scratch, "fml_qk_norm_rope_bwd: gain gradients need the scratch buffer");
+  const long long sw = (long long)MAX_PARTS * 2 * d_head;
+  FML_REQUIRE(ctx, !clash(dgain_q, d_head, d_head, dgain_k, d_head, d_head, 1) && !clash(dgain_q, d_head, d_head, scratch, sw, sw, 1) &&
+                       !clash(dgain_k, d_head, d_head, scratch, sw, sw, 1),
+              "fml_qk_norm_rope_bwd: the gain gradients and the scratch buffer must not overlap");
   if (rows == 0) return FML_OK;
   p.kexp = rot_dim ? -2.0 * log2(base) / rot_dim : 0.0;
   p.parts = dgain_q || dgain_k ? scratch : nullptr;

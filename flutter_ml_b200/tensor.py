@@ -422,7 +422,7 @@ class QKNorm:
 
     @property
     def inputs(self):
-        return [g for g in (self.gain_q, self.gain_k) if g is not None]
+        return [g for g in (self.gain_q, self.gain_k if self.gain_k is not self.gain_q else None) if g is not None]
 
     def _options(self, rows, seq_len, ld):
         if self.positions is not None and (self.positions.dtype != np.int32 or self.positions.size < rows):
@@ -443,10 +443,15 @@ class QKNorm:
             if g.grad is None:
                 g.zeroGrad()
         scratch = ctx.empty(ops.qk_norm_rope_scratch(d_head)) if self.inputs else None
+        dgain_q, dgain_k = (g.grad if g is not None else None for g in (self.gain_q, self.gain_k))
+        shared = dgain_q is not None and self.gain_k is self.gain_q     # one gain for both: two sums, then added
+        if shared:
+            dgain_k = ctx.zeros(d_head)
         ops.qk_norm_rope_backward(ctx, x, x.view(d, ()), dout, dout.view(d, ()), dx, dx.view(d, ()), rows, heads_q, heads_k, d_head,
-                                  dgain_q=self.gain_q.grad if self.gain_q is not None else None,
-                                  dgain_k=self.gain_k.grad if self.gain_k is not None else None, ld_dq_out=ld_dout, ld_dk_out=ld_dout, ld_dq=ld,
-                                  ld_dk=ld, accumulate=accumulate, scratch=scratch, **self._options(rows, seq_len, ld))
+                                  dgain_q=dgain_q, dgain_k=dgain_k if heads_k else None, ld_dq_out=ld_dout, ld_dk_out=ld_dout, ld_dq=ld, ld_dk=ld,
+                                  accumulate=accumulate, scratch=scratch, **self._options(rows, seq_len, ld))
+        if shared:
+            ctx.call("fml_axpy", 1.0, dgain_k, dgain_q, d_head)
 
 
 def qkNormRope(x: Tensor, heads_q: int, heads_k: int, d_head: int, norm: Optional[QKNorm] = None, seq_len: int = 0) -> Tensor:

@@ -350,6 +350,7 @@ int32_t fml_optimizer_step(fml_ctx* ctx, int32_t kind, float* w, const float* g,
  *                be partly unused).  32 bits: m and v, 256 floats a block.  8 bits: first the codes of all blocks, 256
  *                bytes each (sign, 4 exponent and 3 fraction bits, 0x7f NaN), then one float32 scale, a power of two, for
  *                each block; an element is code * scale, and the second buffer holds sqrt(v).
+ * Steps of one plan follow each other (they update the same buffers); different plans may run at once on different lanes.
  * A plan belongs to its context, which frees those that are left at fml_shutdown; it must outlive the graphs that were
  * recorded with it.  Make and destroy plans outside recordings (both wait for the device). */
 int32_t fml_adamw_state_floats(int32_t n, const int64_t* sizes, int32_t state_bits, int64_t* floats);
@@ -490,7 +491,7 @@ int32_t fml_attention_bwd(fml_ctx* ctx, const fml_attention_desc* d, const float
  * nothing else with another buffer.
  * Backward: dq, dk from the forward pass's inputs and the gradients of its outputs, overwritten or added to (accumulate);
  * dgain_q, dgain_k (either may be NULL) are added to, through `scratch` of FML_QK_NORM_ROPE_PARTS * 2 * d_head floats
- * (may be NULL when both are). */
+ * (may be NULL when both are; the three must not overlap). */
 #define FML_QK_NORM_ROPE_PARTS 592
 int32_t fml_qk_norm_rope_fwd(fml_ctx* ctx, const float* q, int64_t ld_q, float* q_out, int64_t ld_q_out, int32_t heads_q,
                              const float* k, int64_t ld_k, float* k_out, int64_t ld_k_out, int32_t heads_k, int64_t rows,
@@ -560,7 +561,7 @@ int32_t fml_lstm_cell_bwd(fml_ctx* ctx, const float* gates, const float* c_prev,
 /* ---- gated linear recurrence ---------------------------------------------------
  * (Extension beside the LSTM: gates that do not read the state, so the steps can be joined in any grouping.)  For every
  * sequence s, channel c and step t < lens[s] (lens NULL: seq_len), from h0 [n_seq][dim] (NULL: zero):
- *   FML_RECURRENCE_GATED   a = sigmoid(f),  h_t = a h_{t-1} + (1 - a) x_t
+ *   FML_RECURRENCE_GATED   a = sigmoid(f),  h_t = a h_{t-1} + (1 - a) x_t   (f below -80 counts as -80)
  *   FML_RECURRENCE_LINEAR  a = f,           h_t = a h_{t-1} + x_t
  * Element (s, t, c) of f and x lies at s * seq_stride_in + t * step_stride_in + c (elements; both arrays share the strides,
  * so they may be the halves of one fused projection), of h at the strides of h: sequence-major, time-major and sliced

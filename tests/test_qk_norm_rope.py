@@ -48,6 +48,18 @@ def reference(x, gain, pos, rot, interleaved, base, eps, dy=None):
     return out
 
 
+def test_dividing_by_multiplying_is_exact_where_it_is_used():
+    """The kernel counts a CTA's heads through and divides by the heads of a row with floor(n ceil(2^32 / h) / 2^32); it takes
+    at most 2^31 / h^2 rows (or one) at a time, so n < 2^31 / h or n < h."""
+    rng = np.random.default_rng(0)
+    for h in [2, 3, 5, 7, 12, 100, 127, 128, 1000, 5792, 5793, 8191, 11585, 11586, 20000, 32767, 32768] + list(rng.integers(2, 32769, 200)):
+        h = int(h)
+        most = h * max(1, min(32, 2 ** 31 // (h * h)))
+        n = np.unique(np.concatenate([np.arange(min(most, 5000)), most - 1 - np.arange(min(most, 5000)), np.arange(h - 1, most, h), np.arange(0, most, h)]))
+        n = n.astype(np.uint64)
+        assert np.array_equal((n * np.uint64(-(-2 ** 32 // h))) >> np.uint64(32), n // np.uint64(h)), h
+
+
 @pytest.fixture(scope="module")
 def ctx():
     from flutter_ml_b200 import _lib
@@ -147,7 +159,8 @@ CASES = [
     dict(rows=31, hq=2, hk=2, d=256, rot=0),
     dict(rows=20000, hq=2, hk=1, d=64, rot=64, positions=512),                    # more rows than one round of CTAs takes
     dict(rows=3001, hq=1, hk=1, d=10, rot=6),
-    dict(rows=77, hq=5, hk=2, d=24, rot=8),                                       # three lanes a head, ten heads a warp
+    dict(rows=77, hq=5, hk=2, d=24, rot=8),
+    dict(rows=1300, hq=700, hk=1, d=8, rot=8, gain=False),                        # many heads, two and three rows a CTA
     dict(rows=201, hq=7, hk=7, d=40, rot=40, shift=2),
     dict(rows=45, hq=9, hk=3, d=72, rot=64, interleaved=True),
     dict(rows=700, hq=1, hk=1, d=16, rot=0),
@@ -316,6 +329,10 @@ def test_refusals(ctx):
             bwd(**bad)
     with pytest.raises(ValueError):
         bwd(gain_q=g, dgain_q=g, scratch=g)
+    for bad in (dict(dgain_k=g), dict(dgain_k=s.view(100, (64,))), dict(dgain_q=s.view(0, (64,)), dgain_k=g)):   # sums into one place
+        with pytest.raises(_lib.FmlError):
+            bwd(**{**dict(k=x.view(64, ()), dk_out=ctx.zeros(8, 256), dk=ctx.zeros(8, 256), heads_k=1, gain_q=g, gain_k=g, dgain_q=g, scratch=s,
+                          ld_k=256, ld_q=256), **bad})
 
 
 @pytest.mark.gpu
@@ -379,6 +396,25 @@ def test_attention_layer_with_norm_and_rotation(ctx, fused, twice):
     for got, want in ((x.grad, tx.grad), (layer.Wqkv.grad, t["w"].grad), (layer.Wo.grad, t["o"].grad), (layer.gainQ.grad, t["gq"].grad),
                       (layer.gainK.grad, t["gk"].grad)):
         assert rel(got.numpy(), want) <= 8e-3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads_k", [0, 2])
+def test_one_gain_for_queries_and_keys(ctx, heads_k):
+    """The same Tensor as both gains (or with no keys): its gradient is the sum of both sides', added once each."""
+    from flutter_ml_b200 import tensor as T
+    rng = np.random.default_rng(6)
+    C = (2 + heads_k) * 32
+    x0, dy, g0 = (rng.standard_normal(s).astype(f32) for s in ((40, C), (40, C), 32))
+    x, g = T.Tensor(x0, ctx), T.Tensor(g0, ctx)
+    y = T.qkNormRope(x, 2, heads_k, 32, T.QKNorm(g, g), seq_len=40)
+    assert y.creator.inputs == [x, g]
+    y.grad = ctx.upload(dy)
+    y.backward()
+    r = reference(x0.reshape(40, -1, 32).astype(np.float64), g0.astype(np.float64), np.arange(40), 32, False, 10000.0, 1e-6,
+                  dy.reshape(40, -1, 32).astype(np.float64))
+    close(g.grad.numpy(), r[4], r[5] + 2 * U * np.abs(r[4]), "gain gradient")
+    close(x.grad.numpy().reshape(40, -1, 32), r[2], r[3], "gradient")
 
 
 @pytest.mark.gpu
