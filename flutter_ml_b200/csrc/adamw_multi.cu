@@ -18,12 +18,17 @@
 // part of it, smaller ones become zero; a positive r is held at 2^-9 of the scale at least, because m over a root that was
 // rounded to zero would be a step of any size.  beta2 = 0.999 changes v by a thousandth a step, far less than the half step
 // of 1/16 that rounding to the nearest takes away, so a v rounded that way stands still until a gradient beats it by an
-// order of magnitude: rounding up with the probability of the dropped bits (16 of them) keeps every state right on average.
+// order of magnitude: rounding up with the probability of the dropped bits (16 of them) keeps m and the root right on average
+// (v, the square of the root, is high by the variance of the rounding: 4 % in a simulation with normal gradients).
 // The bits come from a counter (seed, step, block, element), so a run can be repeated exactly.  An element that is not
 // finite is held as NaN and left out of the block's scale: it damages nothing but itself.
 //
 // The moments are formed with one rounding an operation (no contraction), so a restatement in any IEEE float32 arithmetic
-// reproduces the codes bit for bit.
+// reproduces the codes bit for bit, but for a root that is one unit off (see roots8) at the border of two codes.
+//
+// Measured on 141 M parameters: 32 bits 566 us, 7.0 TB/s; 8 bits 356 us in short runs (6.4 TB/s), 395 in long ones, where the
+// power cap lowers the clock: about 60 instructions an element, 0.8 of the issue slots.  The first form, codes taken apart by
+// shifts and selections, took 549.  Persistent CTAs with the next block in registers: 460 (two CTAs an SM).
 #include <math.h>
 
 #include <algorithm>

@@ -11,13 +11,16 @@
 //
 // Layout: 4, 8, 16 or 32 lanes hold a head (d_head up to 32, 64, 128, 256), eight elements each: two float4, in the rotated
 // part four elements of its first half and their partners of the second, so a pair never leaves its lane; the only exchange
-// is the reduction.  A warp takes 32 / lanes heads of a row at once, queries and keys alike, and its next items' loads go
-// out before the first is used.  The cosines and sines of a CTA's rows are formed once, into shared memory, for all heads:
-// the angle in turns in double (pos times a frequency keeps no fraction in 24 bits at far positions), its fraction in float.
-// Addresses or row strides that float4 cannot take
-// are read float by float in the same places; head widths and rotated parts that are no multiple of eight run the same steps
-// with one warp a head, pairs of floats.
+// is the reduction.  A warp takes 32 / lanes heads at once, the heads of a CTA's rows counted through, and the loads of two
+// such items go out before the first is used.  The cosines and sines of a CTA's rows are formed once, into shared memory, for
+// all heads: the angle in turns in double (pos times a frequency keeps no fraction in 24 bits at far positions), its fraction
+// in float.  Addresses or row strides that float4 cannot take are read float by float in the same places; head widths and
+// rotated parts that are no multiple of eight run the same steps with one warp a head, pairs of floats.
 // dgain: each CTA leaves its sums in the caller's scratch, a second launch adds them in a fixed order.
+//
+// Measured on 16384 rows of 16 + 16 heads of 64: forward 43 us (0.96 of the copy bandwidth), backward 71 (0.87), the gain sums
+// 5.  4999 rows of 12 + 3 heads of 80 at an odd stride: 15 and 27 us (0.5 and 0.4), bound by instructions: ten of sixteen lanes
+// work, with single floats (whole pairs side by side in the lanes, so that neighbours load neighbours, took 17 and 26).
 #include <math.h>
 
 #include <algorithm>
