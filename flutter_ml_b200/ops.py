@@ -179,19 +179,31 @@ def gated_recurrence_forward(ctx, f, x, h, n_seq, seq_len, dim, form="gated", h0
     """h_t = a_t h_{t-1} + (1 - a_t) x_t with a = sigmoid(f) (form "gated"), or h_t = f_t h_{t-1} + x_t ("linear"), along every
     sequence (`fml_gated_recurrence_fwd`).  strides_in (f and x) and strides_h are (sequence, step) strides in elements,
     sequence-major without gaps by default; lens: int32 lengths on the device."""
+    if lens is not None and lens.dtype != np.int32:
+        raise ValueError("gated_recurrence: lens must be int32")
     dense = (seq_len * dim, dim)
     si, sh = strides_in or dense, strides_h or dense
-    ctx.call("fml_gated_recurrence_fwd", _lib.RECURRENCE_BY_NAME[form], n_seq, seq_len, dim, f, x, si[0], si[1], h0, lens, h, sh[0], sh[1], h_last)
+    rc = ctx.lib.fml_gated_recurrence_fwd(ctx.h, _lib.RECURRENCE_BY_NAME[form], n_seq, seq_len, dim, f and f.ptr, x and x.ptr, si[0], si[1],
+                                          h0 and h0.ptr, lens and lens.ptr, h and h.ptr, sh[0], sh[1], h_last and h_last.ptr)
+    if rc:
+        ctx.check(rc)
+    ctx.launches += 1
 
 
 def gated_recurrence_backward(ctx, f, x, h, dy, df, dx, n_seq, seq_len, dim, form="gated", h0=None, lens=None, dh_last=None, dh0=None,
                               strides_in=None, strides_h=None, accumulate=False):
     """Gradients of `gated_recurrence_forward` from its inputs and its h (`fml_gated_recurrence_bwd`); dy may be None (zero),
     df and dx lie at the strides of f and x, dy at those of h."""
+    if lens is not None and lens.dtype != np.int32:
+        raise ValueError("gated_recurrence: lens must be int32")
     dense = (seq_len * dim, dim)
     si, sh = strides_in or dense, strides_h or dense
-    ctx.call("fml_gated_recurrence_bwd", _lib.RECURRENCE_BY_NAME[form], n_seq, seq_len, dim, f, x, si[0], si[1], h0, lens, h, dy, sh[0], sh[1],
-             dh_last, df, dx, dh0, 1 if accumulate else 0)
+    rc = ctx.lib.fml_gated_recurrence_bwd(ctx.h, _lib.RECURRENCE_BY_NAME[form], n_seq, seq_len, dim, f and f.ptr, x and x.ptr, si[0], si[1],
+                                          h0 and h0.ptr, lens and lens.ptr, h and h.ptr, dy and dy.ptr, sh[0], sh[1], dh_last and dh_last.ptr,
+                                          df and df.ptr, dx and dx.ptr, dh0 and dh0.ptr, 1 if accumulate else 0)
+    if rc:
+        ctx.check(rc)
+    ctx.launches += 1
 
 
 def qk_norm_rope_scratch(d_head: int) -> int:
@@ -203,9 +215,15 @@ def qk_norm_rope_forward(ctx, q, k, q_out, k_out, rows, heads_q, heads_k, d_head
                          rot_dim=None, interleaved=False, base=10000.0, eps=1e-6, ld_q=None, ld_k=None, ld_q_out=None, ld_k_out=None):
     """Norm of every query and key head, its gain, and the rotation by position, in one launch (`fml_qk_norm_rope_fwd`).
     Row strides default to rows that lie end to end; rot_dim defaults to the whole head; k may be None with heads_k = 0."""
+    if positions is not None and positions.dtype != np.int32:
+        raise ValueError("qk_norm_rope: positions must be int32")
     wq, wk = heads_q * d_head, heads_k * d_head
-    ctx.call("fml_qk_norm_rope_fwd", q, ld_q or wq, q_out, ld_q_out or wq, heads_q, k, ld_k or wk, k_out, ld_k_out or wk, heads_k, rows, d_head,
-             gain_q, gain_k, positions, seq_len, d_head if rot_dim is None else rot_dim, 1 if interleaved else 0, base, eps)
+    rc = ctx.lib.fml_qk_norm_rope_fwd(ctx.h, q and q.ptr, ld_q or wq, q_out and q_out.ptr, ld_q_out or wq, heads_q, k and k.ptr, ld_k or wk,
+                                      k_out and k_out.ptr, ld_k_out or wk, heads_k, rows, d_head, gain_q and gain_q.ptr, gain_k and gain_k.ptr,
+                                      positions and positions.ptr, seq_len, d_head if rot_dim is None else rot_dim, 1 if interleaved else 0, base, eps)
+    if rc:
+        ctx.check(rc)
+    ctx.launches += 1
 
 
 def qk_norm_rope_backward(ctx, q, k, dq_out, dk_out, dq, dk, rows, heads_q, heads_k, d_head, gain_q=None, gain_k=None, dgain_q=None,
@@ -213,12 +231,19 @@ def qk_norm_rope_backward(ctx, q, k, dq_out, dk_out, dq, dk, rows, heads_q, head
                           ld_k=None, ld_dq_out=None, ld_dk_out=None, ld_dq=None, ld_dk=None, accumulate=False, scratch=None):
     """Gradients of `qk_norm_rope_forward` (`fml_qk_norm_rope_bwd`); dgain_q and dgain_k are added to, through `scratch` of
     `qk_norm_rope_scratch(d_head)` floats."""
+    if positions is not None and positions.dtype != np.int32:
+        raise ValueError("qk_norm_rope: positions must be int32")
     wq, wk = heads_q * d_head, heads_k * d_head
     if scratch is not None and scratch.size < qk_norm_rope_scratch(d_head):
         raise ValueError(f"qk_norm_rope_backward: the scratch buffer needs {qk_norm_rope_scratch(d_head)} floats")
-    ctx.call("fml_qk_norm_rope_bwd", q, ld_q or wq, dq_out, ld_dq_out or wq, dq, ld_dq or wq, heads_q, k, ld_k or wk, dk_out, ld_dk_out or wk, dk,
-             ld_dk or wk, heads_k, rows, d_head, gain_q, gain_k, dgain_q, dgain_k, positions, seq_len, d_head if rot_dim is None else rot_dim,
-             1 if interleaved else 0, base, eps, 1 if accumulate else 0, scratch, launches=2 if dgain_q is not None or dgain_k is not None else 1)
+    rc = ctx.lib.fml_qk_norm_rope_bwd(ctx.h, q and q.ptr, ld_q or wq, dq_out and dq_out.ptr, ld_dq_out or wq, dq and dq.ptr, ld_dq or wq, heads_q,
+                                      k and k.ptr, ld_k or wk, dk_out and dk_out.ptr, ld_dk_out or wk, dk and dk.ptr, ld_dk or wk, heads_k, rows,
+                                      d_head, gain_q and gain_q.ptr, gain_k and gain_k.ptr, dgain_q and dgain_q.ptr, dgain_k and dgain_k.ptr,
+                                      positions and positions.ptr, seq_len, d_head if rot_dim is None else rot_dim, 1 if interleaved else 0, base,
+                                      eps, 1 if accumulate else 0, scratch and scratch.ptr)
+    if rc:
+        ctx.check(rc)
+    ctx.launches += 2 if dgain_q is not None or dgain_k is not None else 1
 
 
 class AdamWPlan:

@@ -379,6 +379,8 @@ def test_refusals(ctx):
             fwd(**bad)
     with pytest.raises(KeyError):
         fwd(form="other")
+    with pytest.raises(ValueError):
+        fwd(lens=at(3 * n))
     with pytest.raises(_lib.FmlError):
         ctx.call("fml_gated_recurrence_fwd", 2, 2, 5, 8, at(0), at(n), 40, 8, None, None, at(2 * n), 40, 8, None)
 

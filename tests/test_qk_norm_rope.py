@@ -318,6 +318,9 @@ def test_refusals(ctx):
         with pytest.raises(_lib.FmlError):
             fwd(**bad)
 
+    with pytest.raises(ValueError):
+        fwd(positions=ctx.zeros(8))
+
     def bwd(**kw):
         a = dict(q=x, k=None, dq_out=y, dk_out=None, dq=y, dk=None, rows=8, heads_q=1, heads_k=0, d_head=64)
         a.update(kw)
