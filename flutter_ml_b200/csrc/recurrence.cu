@@ -21,11 +21,13 @@
 //
 // Measured (us; bytes at the copy's rate in brackets): 128 sequences of 128 x 512 forward 18 (15); 32 ragged ones of 512 x 1024
 // 21 forward (14), 37 backward (29); 8 of 2048 x 1024 36 (31) and 69 (61); one of 16384 x 1024, in clusters of four, 44 (31) and
-// 78 (61); one of 65521 x 250, in clusters of eight, LINEAR, 61 (30) and 97 (50).  The first are bound by memory, with about 5 us
+// 78 (61); one of 65521 x 250, in clusters of eight, LINEAR, 61 (30) and 97 (50); one of 52433 x 192, in clusters of sixteen, 42
+// (18) and 73 (37).  The first are bound by memory, with about 5 us
 // for the first loads and last stores; the clusters by the chain of a round, which 16 warps an SM do not hide.
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdlib>
 
 #include "common.cuh"
@@ -34,7 +36,7 @@
 namespace {
 
 constexpr int THREADS = 256;
-constexpr int MAX_CLUSTER = 8;
+constexpr int MAX_CLUSTER = 16;   // above 8 where the device says that such a cluster fits
 constexpr int WAIT_CODE = 130;   // fml_device_status: a cluster's pairs did not arrive
 
 struct Params {
@@ -488,28 +490,84 @@ int vector_width(const Params& p) {
   return (all & 15) == 0 && n % 4 == 0 ? 4 : (all & 7) == 0 && n % 2 == 0 ? 2 : 1;
 }
 
+// Largest cluster of this kernel: 8, or 16 where the device can hold one; asked for once a device.
+template <int LANES, int VEC, int SEG, bool GATED, bool BWD>
+int32_t largest_cluster(fml_ctx* ctx, int* out) {
+  static std::atomic<int> known[FML_MAX_DEVICES];
+  const bool slot = ctx->device >= 0 && ctx->device < FML_MAX_DEVICES;
+  int n = slot ? known[ctx->device].load(std::memory_order_acquire) : 0;
+  if (n == 0) {
+    auto* kernel = scan_kernel<8, LANES, VEC, SEG, GATED, BWD, false, true>;
+    FML_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(MAX_CLUSTER);
+    cfg.blockDim = dim3(256);
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim = {MAX_CLUSTER, 1, 1};
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int fit = 0;
+    if (cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg) != cudaSuccess) {
+      fit = 0;
+      (void)cudaGetLastError();
+    }
+    n = fit > 0 ? MAX_CLUSTER : 8;
+    if (slot) known[ctx->device].store(n, std::memory_order_release);
+  }
+  *out = n;
+  return FML_OK;
+}
+
+// Few channels: eight warps, rows of LANES, long segments forward, and a cluster along the steps: two CTAs an SM, or where eight
+// CTAs a cluster do not give one an SM, up to sixteen and one and a half; no more of them than the same number of rounds needs.
+// One sequence of 65521 x 250: 61 and 97 us with eight CTAs, of 16384 x 1024: 44 and 78 with four, of 52433 x 192: 42 and 74 with
+// sixteen (56 and 105 with eight), of 18285 x 256: 21 and 37 with twelve (27 and 44).
+template <int LANES, int VEC, bool GATED, bool BWD>
+int32_t launch_team(fml_ctx* ctx, Params& p) {
+  constexpr int SEG = (BWD ? 16 : 32) / VEC, TILE = 8 * (32 / LANES) * SEG;
+  const long long units = (long long)p.n_seq * ((p.dim + LANES * VEC - 1) / (LANES * VEC)), sms = ctx->sm_count;
+  long long cluster = std::min(8ll, 2 * sms / units);
+  if (units * 8 < sms) {
+    int most = 8;
+    const int32_t rc = largest_cluster<LANES, VEC, SEG, GATED, BWD>(ctx, &most);
+    if (rc) return rc;
+    cluster = std::min<long long>(most, 3 * sms / 2 / units);
+  }
+  if (cluster > 1) {
+    const long long rounds = (p.seq_len + TILE * cluster - 1) / (TILE * cluster);
+    cluster = (p.seq_len + TILE * rounds - 1) / (TILE * rounds);
+  }
+  if (cluster > 1) return launch_scan<8, LANES, VEC, SEG, GATED, BWD, false, true>(ctx, p, (int)cluster);
+  return launch_scan<8, LANES, VEC, SEG, GATED, BWD, false, false>(ctx, p, 1);
+}
+
 template <int VEC, bool GATED, bool BWD>
 int32_t launch_lanes(fml_ctx* ctx, Params& p) {
   constexpr int SEG = 16 / VEC;
   auto units = [&](int lanes) { return (long long)p.n_seq * ((p.dim + lanes * VEC - 1) / (lanes * VEC)); };
   const int sms = ctx->sm_count;
-  // Channels enough: each CTA goes over all steps of its channels, the next round's rows in registers meanwhile; rows of 32
-  // lanes where that leaves three CTAs of four warps an SM, else of 16 or 8 (before the last steps, 128 sequences of 128 x 512:
-  // 21.2 us forward and 38 backward with 32 lanes, 21.6 and 40 with 16; 32 ragged ones of 512 x 1024: 23.4 and 40.6 with 8, 25.6
-  // and 40.7 with 16),
-  // CTAs of eight warps where there are few (8 of 2048 x 1024: 36 and 70; four warps 46 and 70, clusters 57 and 118).
-  if (units(32) >= 3 * sms) return launch_scan<4, 32, VEC, SEG, GATED, BWD, true, false>(ctx, p, 1);
-  if (units(16) >= 4 * sms) return launch_scan<4, 16, VEC, SEG, GATED, BWD, true, false>(ctx, p, 1);
-  if (units(8) >= 4 * sms) return launch_scan<4, 8, VEC, SEG, GATED, BWD, true, false>(ctx, p, 1);
-  if (units(8) >= sms) return launch_scan<8, 8, VEC, SEG, GATED, BWD, true, false>(ctx, p, 1);
-  // Few: eight warps, rows of four lanes, long segments forward, and a cluster along the steps that gives two CTAs an SM (one
-  // sequence of 65521 x 250: 61 and 97 us with eight CTAs; rows of eight lanes, half the CTAs, 91 and 135; one of 16384 x 1024:
-  // 44 and 78 with four).
-  constexpr int LONG = BWD ? SEG : 2 * SEG;
-  int cluster = (int)std::min<long long>(MAX_CLUSTER, 2 * sms / units(4));
-  while (cluster > 1 && 64ll * LONG * (cluster - 1) >= p.seq_len) cluster--;   // every CTA has steps
-  if (cluster > 1) return launch_scan<8, 4, VEC, LONG, GATED, BWD, false, true>(ctx, p, cluster);
-  return launch_scan<8, 4, VEC, LONG, GATED, BWD, false, false>(ctx, p, 1);
+  // Channels enough: each CTA goes over all steps of its channels, the next round's rows in registers meanwhile.  Rows as wide as
+  // leave three to four CTAs of four warps an SM, at least 32 channels of them, else eight warps.  Measured (us, forward and
+  // backward): 128 sequences of 128 x 512, 32 lanes of four: 18 and 35.  32 of 512 x 1024: 34 and 65 with 16 lanes, 35 and 68
+  // with 8; ragged 25 and 37, 21 and 37.  8 of 2048 x 1024, eight warps of 8 lanes: 36 and 69, four warps 49 and 68.  Two
+  // channels a lane, 8 of 2048 x 1022: eight warps of 16 lanes 37 and 74, of 8 40 and 84.  One, 32 of 512 x 1001: 32 lanes 39
+  // and 84, 8 46 and 108; 100 of 300 x 77: 16 lanes 10 and 20, 8 13 and 29.
+#define FML_SCAN(warps, lanes) return launch_scan<warps, lanes, VEC, SEG, GATED, BWD, true, false>(ctx, p, 1)
+  if (VEC == 4) {
+    if (units(32) >= 3 * sms) FML_SCAN(4, 32);
+    if (units(16) >= (p.lens ? 4 : 3) * sms) FML_SCAN(4, 16);
+    if (units(8) >= 4 * sms) FML_SCAN(4, 8);
+  } else {
+    if (units(32) >= 4 * sms) FML_SCAN(4, 32);
+    if (units(16) >= (VEC == 2 ? 4 : 3) * sms) FML_SCAN(4, 16);
+    if (2 * units(16) >= (VEC == 2 ? 3 : 2) * sms) FML_SCAN(8, 16);
+  }
+  if (units(8) >= sms) FML_SCAN(8, 8);
+#undef FML_SCAN
+  if (VEC == 1) return launch_team<8, VEC, GATED, BWD>(ctx, p);
+  if (VEC == 4 && units(4) * MAX_CLUSTER < sms) return launch_team<2, VEC, GATED, BWD>(ctx, p);   // rows of one sector
+  return launch_team<4, VEC, GATED, BWD>(ctx, p);
 }
 
 template <bool GATED, bool BWD>

@@ -155,7 +155,7 @@ def close(got, ref, bound, what):
 
 
 SIZES = [(1, 1, 1), (128, 1, 512), (3, 2, 33), (2, 4, 70), (2, 5, 5), (1, 16, 32), (3, 17, 31), (2, 129, 64), (5, 127, 40), (80, 300, 32),
-         (40, 257, 65), (5, 1000, 64), (3, 2049, 24), (1, 5000, 8), (1, 9001, 1), (1, 4097, 250), (300, 130, 96), (2, 700, 600)]
+         (40, 257, 65), (5, 1000, 64), (3, 2049, 24), (1, 5000, 8), (1, 9001, 1), (1, 4097, 250), (300, 130, 96), (2, 700, 600), (1, 20000, 64), (1, 13000, 130), (40, 60, 130), (50, 40, 33), (3, 150, 1667)]
 
 
 @pytest.mark.gpu
