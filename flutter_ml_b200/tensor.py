@@ -424,7 +424,9 @@ class QKNorm:
     def inputs(self):
         return [g for g in (self.gain_q, self.gain_k if self.gain_k is not self.gain_q else None) if g is not None]
 
-    def _options(self, rows, seq_len, ld):
+    def _options(self, rows, seq_len, d_head, ld):
+        if any(g.value.size != d_head for g in self.inputs):
+            raise ValueError(f"QKNorm: the gains must have the {d_head} elements of a head")
         if self.positions is not None and (self.positions.dtype != np.int32 or self.positions.size < rows):
             raise ValueError("QKNorm: positions must be int32, one for each row")
         return dict(gain_q=self.gain_q.value if self.gain_q is not None else None, gain_k=self.gain_k.value if self.gain_k is not None else None,
@@ -435,7 +437,7 @@ class QKNorm:
         """x, out: buffers with the queries in their first heads_q * d_head columns and the keys behind them."""
         d = heads_q * d_head
         ops.qk_norm_rope_forward(ctx, x, x.view(d, ()), out, out.view(d, ()), rows, heads_q, heads_k, d_head, ld_q_out=ld_out, ld_k_out=ld_out,
-                                 **self._options(rows, seq_len, ld))
+                                 **self._options(rows, seq_len, d_head, ld))
 
     def backward(self, ctx, x, dout, dx, rows, seq_len, heads_q, heads_k, d_head, ld, ld_dout, accumulate):
         d = heads_q * d_head
@@ -449,7 +451,7 @@ class QKNorm:
             dgain_k = ctx.zeros(d_head)
         ops.qk_norm_rope_backward(ctx, x, x.view(d, ()), dout, dout.view(d, ()), dx, dx.view(d, ()), rows, heads_q, heads_k, d_head,
                                   dgain_q=dgain_q, dgain_k=dgain_k if heads_k else None, ld_dq_out=ld_dout, ld_dk_out=ld_dout, ld_dq=ld, ld_dk=ld,
-                                  accumulate=accumulate, scratch=scratch, **self._options(rows, seq_len, ld))
+                                  accumulate=accumulate, scratch=scratch, **self._options(rows, seq_len, d_head, ld))
         if shared:
             ctx.call("fml_axpy", 1.0, dgain_k, dgain_q, d_head)
 

@@ -60,6 +60,23 @@ def test_dividing_by_multiplying_is_exact_where_it_is_used():
         assert np.array_equal((n * np.uint64(-(-2 ** 32 // h))) >> np.uint64(32), n // np.uint64(h)), h
 
 
+def test_gains_of_another_head_width_are_refused():
+    """The kernels read d_head elements of each gain, so a shorter one must not get that far."""
+    from types import SimpleNamespace
+    from flutter_ml_b200 import tensor as T
+    gain = lambda n: SimpleNamespace(value=SimpleNamespace(size=n, shape=(n,)))  # noqa: E731
+    for gq, gk in ((gain(63), None), (None, gain(63)), (gain(64), gain(128))):
+        norm, x = T.QKNorm(gq, gk), SimpleNamespace(view=lambda *a: None)
+        with pytest.raises(ValueError):
+            norm.forward(None, x, x, 4, 4, 2, 2, 64, 256, 256)
+        gradient = SimpleNamespace(grad=0)
+        for g in norm.inputs:
+            g.grad = gradient
+        ctx = SimpleNamespace(empty=lambda *a: None)
+        with pytest.raises(ValueError):
+            norm.backward(ctx, x, x, x, 4, 4, 2, 2, 64, 256, 256, False)
+
+
 @pytest.fixture(scope="module")
 def ctx():
     from flutter_ml_b200 import _lib
