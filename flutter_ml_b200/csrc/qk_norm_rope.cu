@@ -11,15 +11,15 @@
 //
 // Layout: 4, 8, 16 or 32 lanes hold a head (d_head up to 32, 64, 128, 256), eight elements each: two float4, in the rotated
 // part four elements of its first half and their partners of the second, so a pair never leaves its lane; the only exchange
-// is the reduction.  A warp takes 32 / lanes heads at once, the heads of a CTA's rows counted through, and the loads of two
-// such items go out before the first is used.  The cosines and sines of a CTA's rows are formed once, into shared memory, for
+// is the reduction.  A warp takes 32 / lanes heads at once, the heads of a CTA's rows counted through, and the loads of the
+// next such item are under way while one is used.  The cosines and sines of a CTA's rows are formed once, into shared memory, for
 // all heads: the angle in turns in double (pos times a frequency keeps no fraction in 24 bits at far positions), its fraction
 // in float.  Addresses or row strides that float4 cannot take are read float by float in the same places; head widths and
 // rotated parts that are no multiple of eight run the same steps with one warp a head, pairs of floats.
 // dgain: each CTA leaves its sums in the caller's scratch, a second launch adds them in a fixed order.
 //
-// Measured on 16384 rows of 16 + 16 heads of 64: forward 43 us (0.96 of the copy bandwidth), backward 71 (0.87), the gain sums
-// 5.  4999 rows of 12 + 3 heads of 80 at an odd stride: 15 and 27 us (0.5 and 0.4), bound by instructions: ten of sixteen lanes
+// Measured on 16384 rows of 16 + 16 heads of 64: forward 47 us (0.88 of the copy bandwidth), backward 66 (0.93), the gain sums
+// 5.  4999 rows of 12 + 3 heads of 80 at an odd stride: 14 and 21 us (0.5 of it), bound by instructions: ten of sixteen lanes
 // work, with single floats (whole pairs side by side in the lanes, so that neighbours load neighbours, took 17 and 26).
 #include <math.h>
 
@@ -32,9 +32,9 @@ namespace {
 constexpr int WARPS = 8, THREADS = 32 * WARPS;
 constexpr int MAX_PARTS = FML_QK_NORM_ROPE_PARTS;   // CTAs of a backward launch, one partial sum each
 constexpr int MAX_D = 256;
-// CTAs an SM: 64 registers a thread forward, 128 backward.  Measured on 16384 rows of 16 + 16 heads of 64, both passes: 129 us;
-// backward with three (80 registers, spills) or four items' loads in flight forward (three CTAs): 140 us.
-constexpr int CTAS_FWD = 4, CTAS_BWD = 2;
+// CTAs an SM: 64 registers a thread forward, 80 backward.  Measured on 16384 rows of 16 + 16 heads of 64, both passes: 122 us,
+// 127 with two backward, 129 with five forward; 131 with two items read ahead (three and one CTAs), 129 with CTAs of 16 warps.
+constexpr int CTAS_FWD = 4, CTAS_BWD = 3;
 
 struct Side {          // queries or keys
   const float* x;
@@ -134,88 +134,91 @@ __device__ __forceinline__ void turn8(float* z, const float* cosr, const float* 
   }
 }
 
-// The heads of one side (queries or keys) in rows [r0, r0 + n): counted through, HPW of them a warp's item.
+// A lane's share of a head, read ahead: eight elements, and where they are (row of the CTA's rows, column).
+template <bool BWD>
+struct Item {
+  float x[8], dy[BWD ? 8 : 1];
+  int row, col;
+};
+// Heads it .. it + 32 / LPH - 1 of the side, its heads in rows [r0, r0 + n) counted through.
+template <int LPH, bool BWD>
+__device__ __forceinline__ void load_item(const Params& p, const Side& s, long long r0, int n, int it, const Place& at, Item<BWD>& v) {
+  const int head = it + (threadIdx.x & 31) / LPH;
+  v.row = s.heads == 1 ? head : (int)__umulhi((uint32_t)head, s.per_head);
+  v.col = (head - v.row * s.heads) * p.d;
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    v.x[i] = 0.f;
+    if (BWD) v.dy[i] = 0.f;
+  }
+  if (!at.active || head >= n * s.heads) return;
+  const bool wx = s.wide & 1, wy = s.wide & 2;
+  const float* src = s.x + r0 * s.ldx + v.row * s.ldx + v.col;
+  load4(v.x, src + at.e0, wx);
+  load4(v.x + 4, src + at.e1, wx);
+  if (BWD) {
+    src = s.dy + r0 * s.ldy + v.row * s.ldy + v.col;
+    load4(v.dy, src + at.e0, wy);
+    load4(v.dy + 4, src + at.e1, wy);
+  }
+}
+
+// The heads of one side (queries or keys) in rows [r0, r0 + n), 32 / LPH of them a warp's item; the warp's first item is in
+// `ahead`, and afterwards its first of `then`, the other side, if there is one.
 template <int LPH, bool BWD, bool INTER>
-__device__ __forceinline__ void side_heads(const Params& p, const Side& s, long long r0, int n, const float* cosv, const float* sinv,
-                                           const Place& at, float* dg) {
-  constexpr int HPW = 32 / LPH, U = 2;                // heads of an item; items whose loads go out together
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane / LPH;
-  const int total = n * s.heads, d = p.d;
-  const bool wx = s.wide & 1, wy = s.wide & 2, wo = s.wide & 4;
-  const float inv_d = 1.f / (float)d;
-  const float* x0 = s.x + r0 * s.ldx;
-  const float* y0 = s.dy + r0 * s.ldy;
+__device__ __forceinline__ void side_heads(const Params& p, const Side& s, const Side* then, long long r0, int n, const float* cosv,
+                                           const float* sinv, const Place& at, float* dg, Item<BWD>& ahead) {
+  constexpr int STEP = WARPS * (32 / LPH);
+  const int sub = (threadIdx.x & 31) / LPH, start = (threadIdx.x >> 5) * (32 / LPH);
+  const int total = n * s.heads;
+  const bool wo = s.wide & 4;
+  const float inv_d = 1.f / (float)p.d;
   float* o0 = s.out + r0 * s.ldo;
   float gain[8];
 #pragma unroll
   for (int i = 0; i < 8; i++) gain[i] = at.active && s.gain ? __ldg(s.gain + (i < 4 ? at.e0 : at.e1) + (i & 3)) : 1.f;
-  for (int it = warp * HPW; it < total; it += WARPS * HPW * U) {
-    float x[U][8], dy[BWD ? U : 1][8];
-    int row[U], col[U];
+  if (start >= total && then) load_item<LPH, BWD>(p, *then, r0, n, start, at, ahead);
+  for (int it = start; it < total; it += STEP) {
+    Item<BWD> v = ahead;
+    if (it + STEP < total) load_item<LPH, BWD>(p, s, r0, n, it + STEP, at, ahead);
+    else if (then) load_item<LPH, BWD>(p, *then, r0, n, start, at, ahead);
+    float ss = 0.f;
 #pragma unroll
-    for (int k = 0; k < U; k++) {
-      const int head = it + k * WARPS * HPW + sub;
-      row[k] = s.heads == 1 ? head : (int)__umulhi((uint32_t)head, s.per_head);
-      col[k] = (head - row[k] * s.heads) * d;
+    for (int i = 0; i < 8; i++) ss = fmaf(v.x[i], v.x[i], ss);
+    const float rstd = inv_root(fmaf(head_sum<LPH>(ss), inv_d, p.eps));
+    const int table = min(v.row, n - 1) * at.half;
+    float z[8];
+    if (!BWD) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) z[i] = v.x[i] * rstd * gain[i];
+      if (at.turned) turn8<INTER>(z, cosv + table, sinv + table, at, 1.f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) z[i] = v.dy[i];
+      if (at.turned) turn8<INTER>(z, cosv + table, sinv + table, at, -1.f);
+      float dot = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        x[k][i] = 0.f;
-        if (BWD) dy[k][i] = 0.f;
+        v.x[i] *= rstd;
+        dg[i] = fmaf(z[i], v.x[i], dg[i]);
+        z[i] *= gain[i];
+        dot = fmaf(z[i], v.x[i], dot);
       }
-      if (at.active && head < total) {
-        const float* src = x0 + row[k] * s.ldx + col[k];
-        load4(x[k], src + at.e0, wx);
-        load4(x[k] + 4, src + at.e1, wx);
-        if (BWD) {
-          src = y0 + row[k] * s.ldy + col[k];
-          load4(dy[k], src + at.e0, wy);
-          load4(dy[k] + 4, src + at.e1, wy);
-        }
-      }
+      dot = head_sum<LPH>(dot) * inv_d;
+#pragma unroll
+      for (int i = 0; i < 8; i++) z[i] = rstd * (z[i] - v.x[i] * dot);
     }
+    if (!at.active || it + sub >= total) continue;
+    float* dst = o0 + v.row * s.ldo + v.col;
+    if (BWD && p.accumulate) {
+      float old[8];
+      load4(old, dst + at.e0, wo);
+      load4(old + 4, dst + at.e1, wo);
 #pragma unroll
-    for (int k = 0; k < U; k++) {
-      const int first = it + k * WARPS * HPW;
-      if (first >= total) break;                      // the same for the whole warp
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; i++) ss = fmaf(x[k][i], x[k][i], ss);
-      const float rstd = inv_root(fmaf(head_sum<LPH>(ss), inv_d, p.eps));
-      const int table = min(row[k], n - 1) * at.half;
-      float z[8];
-      if (!BWD) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) z[i] = x[k][i] * rstd * gain[i];
-        if (at.turned) turn8<INTER>(z, cosv + table, sinv + table, at, 1.f);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) z[i] = dy[k][i];
-        if (at.turned) turn8<INTER>(z, cosv + table, sinv + table, at, -1.f);
-        float dot = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          x[k][i] *= rstd;
-          dg[i] = fmaf(z[i], x[k][i], dg[i]);
-          z[i] *= gain[i];
-          dot = fmaf(z[i], x[k][i], dot);
-        }
-        dot = head_sum<LPH>(dot) * inv_d;
-#pragma unroll
-        for (int i = 0; i < 8; i++) z[i] = rstd * (z[i] - x[k][i] * dot);
-      }
-      if (at.active && first + sub < total) {
-        float* dst = o0 + row[k] * s.ldo + col[k];
-        if (BWD && p.accumulate) {
-          float old[8];
-          load4(old, dst + at.e0, wo);
-          load4(old + 4, dst + at.e1, wo);
-#pragma unroll
-          for (int i = 0; i < 8; i++) z[i] += old[i];
-        }
-        store4(dst + at.e0, z, wo);
-        store4(dst + at.e1, z + 4, wo);
-      }
+      for (int i = 0; i < 8; i++) z[i] += old[i];
     }
+    store4(dst + at.e0, z, wo);
+    store4(dst + at.e1, z + 4, wo);
   }
 }
 
@@ -245,11 +248,13 @@ __global__ void __launch_bounds__(THREADS, BWD ? CTAS_BWD : CTAS_FWD) qk_vec_ker
   const long long last = share(p, blockIdx.x + 1);
   for (long long r0 = share(p, blockIdx.x); r0 < last; r0 += p.rows_cta) {
     const int n = (int)min((long long)p.rows_cta, last - r0);
+    Item<BWD> ahead;                                  // under way while the angles are formed
+    load_item<LPH, BWD>(p, p.s[0], r0, n, warp * (32 / LPH), at, ahead);
     __syncthreads();                                  // the table of the step before has been read
     angles(p, freq, r0, n, cosv, sinv);
     __syncthreads();
-    side_heads<LPH, BWD, INTER>(p, p.s[0], r0, n, cosv, sinv, at, dg[0]);
-    side_heads<LPH, BWD, INTER>(p, p.s[1], r0, n, cosv, sinv, at, dg[1]);
+    side_heads<LPH, BWD, INTER>(p, p.s[0], &p.s[1], r0, n, cosv, sinv, at, dg[0], ahead);
+    side_heads<LPH, BWD, INTER>(p, p.s[1], nullptr, r0, n, cosv, sinv, at, dg[1], ahead);
   }
   if (!BWD || !p.parts) return;
   // the CTA's sums: over the warp's heads, then over the warps, in a fixed order
@@ -398,6 +403,11 @@ __global__ void __launch_bounds__(1024) qk_gain_kernel(const float* __restrict__
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
   fml_chain_next();
   fml_chain_wait();
+  const int col = blockIdx.x * 32 + warp;
+  float* dst = col < d ? dgain_q : dgain_k;
+  if (dst) dst += col < d ? col : col - d;
+  const bool mine = lane == 0 && col < 2 * d && dst;
+  const float old = mine ? *dst : 0.f;
   constexpr int PER = (MAX_PARTS + 31) / 32;
   float v[PER], sum = 0.f;
 #pragma unroll
@@ -412,10 +422,7 @@ __global__ void __launch_bounds__(1024) qk_gain_kernel(const float* __restrict__
   sum = red[warp][lane];                              // column `warp` of the block, the warps' sums across the lanes
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const int col = blockIdx.x * 32 + warp;
-  if (lane != 0 || col >= 2 * d) return;
-  float* dst = col < d ? dgain_q : dgain_k;
-  if (dst) dst[col < d ? col : col - d] += sum;
+  if (mine) *dst = old + sum;
 }
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
