@@ -490,21 +490,21 @@ int vector_width(const Params& p) {
   return (all & 15) == 0 && n % 4 == 0 ? 4 : (all & 7) == 0 && n % 2 == 0 ? 2 : 1;
 }
 
-// Largest cluster of this kernel: 8, or 16 where the device can hold one; asked for once a device.
+// How many clusters of this size the device holds at once (none where it cannot form one); asked for once a device and size.
 template <int LANES, int VEC, int SEG, bool GATED, bool BWD>
-int32_t largest_cluster(fml_ctx* ctx, int* out) {
-  static std::atomic<int> known[FML_MAX_DEVICES];
+int32_t clusters_at_once(fml_ctx* ctx, int size, long long* out) {
+  static std::atomic<int> known[FML_MAX_DEVICES][MAX_CLUSTER + 1];   // one more than the answer
   const bool slot = ctx->device >= 0 && ctx->device < FML_MAX_DEVICES;
-  int n = slot ? known[ctx->device].load(std::memory_order_acquire) : 0;
+  int n = slot ? known[ctx->device][size].load(std::memory_order_acquire) : 0;
   if (n == 0) {
     auto* kernel = scan_kernel<8, LANES, VEC, SEG, GATED, BWD, false, true>;
     FML_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(MAX_CLUSTER);
+    cfg.gridDim = dim3(size);
     cfg.blockDim = dim3(256);
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim = {MAX_CLUSTER, 1, 1};
+    at[0].val.clusterDim = {(unsigned)size, 1, 1};
     cfg.attrs = at;
     cfg.numAttrs = 1;
     int fit = 0;
@@ -512,31 +512,31 @@ int32_t largest_cluster(fml_ctx* ctx, int* out) {
       fit = 0;
       (void)cudaGetLastError();
     }
-    n = fit > 0 ? MAX_CLUSTER : 8;
-    if (slot) known[ctx->device].store(n, std::memory_order_release);
+    n = std::max(fit, 0) + 1;
+    if (slot) known[ctx->device][size].store(n, std::memory_order_release);
   }
-  *out = n;
+  *out = n - 1;
   return FML_OK;
 }
 
 // Few channels: eight warps, rows of LANES, long segments forward, and a cluster along the steps: two CTAs an SM, or where eight
-// CTAs a cluster do not give one an SM, up to sixteen and one and a half; no more of them than the same number of rounds needs.
+// CTAs a cluster do not give one an SM, up to sixteen and one and a half; no more of them than the same number of rounds needs,
+// and only as many as let all clusters run at once.
 // One sequence of 65521 x 250: 61 and 97 us with eight CTAs, of 16384 x 1024: 44 and 78 with four, of 52433 x 192: 42 and 74 with
 // sixteen (56 and 105 with eight), of 18285 x 256: 21 and 37 with twelve (27 and 44).
 template <int LANES, int VEC, bool GATED, bool BWD>
 int32_t launch_team(fml_ctx* ctx, Params& p) {
   constexpr int SEG = (BWD ? 16 : 32) / VEC, TILE = 8 * (32 / LANES) * SEG;
   const long long units = (long long)p.n_seq * ((p.dim + LANES * VEC - 1) / (LANES * VEC)), sms = ctx->sm_count;
-  long long cluster = std::min(8ll, 2 * sms / units);
-  if (units * 8 < sms) {
-    int most = 8;
-    const int32_t rc = largest_cluster<LANES, VEC, SEG, GATED, BWD>(ctx, &most);
-    if (rc) return rc;
-    cluster = std::min<long long>(most, 3 * sms / 2 / units);
-  }
-  if (cluster > 1) {
+  long long cluster = units * 8 < sms ? std::min<long long>(MAX_CLUSTER, 3 * sms / 2 / units) : std::min(8ll, 2 * sms / units);
+  for (; cluster > 1; cluster--) {
     const long long rounds = (p.seq_len + TILE * cluster - 1) / (TILE * cluster);
     cluster = (p.seq_len + TILE * rounds - 1) / (TILE * rounds);
+    if (cluster == 1) break;
+    long long fit;
+    const int32_t rc = clusters_at_once<LANES, VEC, SEG, GATED, BWD>(ctx, (int)cluster, &fit);
+    if (rc) return rc;
+    if (units <= fit) break;
   }
   if (cluster > 1) return launch_scan<8, LANES, VEC, SEG, GATED, BWD, false, true>(ctx, p, (int)cluster);
   return launch_scan<8, LANES, VEC, SEG, GATED, BWD, false, false>(ctx, p, 1);
