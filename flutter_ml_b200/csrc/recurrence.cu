@@ -563,11 +563,20 @@ int32_t launch_lanes(fml_ctx* ctx, Params& p) {
     if (units(16) >= (VEC == 2 ? 4 : 3) * sms) FML_SCAN(4, 16);
     if (2 * units(16) >= (VEC == 2 ? 3 : 2) * sms) FML_SCAN(8, 16);
   }
+  if constexpr (BWD) {
+    // A CTA of eight warps fills an SM: few more of them than SMs, and a second wave would go nearly empty.  6 of 3000 x 800
+    // 78 us for 88, 8 of 2500 x 800 the other way 86 and 75; single floats, 10 of 3000 x 197: 39 for 44.
+    if (units(8) >= sms && 4 * units(8) < (VEC == 1 ? 7 : 5) * sms) return launch_team<16, VEC, GATED, BWD>(ctx, p);
+  }
   if (units(8) >= sms) FML_SCAN(8, 8);
 #undef FML_SCAN
-  if (VEC == 1) return launch_team<8, VEC, GATED, BWD>(ctx, p);
-  if (VEC == 4 && units(4) * MAX_CLUSTER < sms) return launch_team<2, VEC, GATED, BWD>(ctx, p);   // rows of one sector
-  return launch_team<4, VEC, GATED, BWD>(ctx, p);
+  if constexpr (VEC == 4) {
+    if (units(4) * MAX_CLUSTER < sms) return launch_team<2, VEC, GATED, BWD>(ctx, p);   // rows of one sector
+    // rows of two sectors, as long as two CTAs share a sequence (one of 9000 x 2600 with four lanes 73 and 215 us, with eight
+    // 62 and 114; of 6618 x 1472 the other way 35 and 59, 31 and 49)
+    if (units(4) <= sms) return launch_team<4, VEC, GATED, BWD>(ctx, p);
+  }
+  return launch_team<8, VEC, GATED, BWD>(ctx, p);
 }
 
 template <bool GATED, bool BWD>
