@@ -21,9 +21,9 @@
 //
 // Measured (us; bytes at the copy's rate in brackets): 128 sequences of 128 x 512 forward 18 (15); 32 ragged ones of 512 x 1024
 // 21 forward (14), 37 backward (29); 8 of 2048 x 1024 36 (31) and 69 (61); one of 16384 x 1024, in clusters of four, 44 (31) and
-// 78 (61); one of 65521 x 250, in clusters of eight, LINEAR, 61 (30) and 97 (50); one of 52433 x 192, in clusters of sixteen, 42
-// (18) and 73 (37).  The first are bound by memory, with about 5 us
-// for the first loads and last stores; the clusters by the chain of a round, which 16 warps an SM do not hide.
+// 78 (61); one of 65521 x 250, in clusters of thirteen, LINEAR, 58 (30) and 96 (50); one of 52433 x 192, in clusters of sixteen,
+// 42 (18) and 73 (37).  The first are bound by memory, with about 5 us for the first loads and last stores; the clusters by the
+// chain of a round, which 16 warps an SM do not hide.
 #include <math.h>
 
 #include <algorithm>
@@ -522,8 +522,9 @@ int32_t clusters_at_once(fml_ctx* ctx, int size, long long* out) {
 // Few channels: eight warps, rows of LANES, long segments forward, and a cluster along the steps: two CTAs an SM, or where eight
 // CTAs a cluster do not give one an SM, up to sixteen and one and a half; no more of them than the same number of rounds needs,
 // and only as many as let all clusters run at once.
-// One sequence of 65521 x 250: 61 and 97 us with eight CTAs, of 16384 x 1024: 44 and 78 with four, of 52433 x 192: 42 and 74 with
-// sixteen (56 and 105 with eight), of 18285 x 256: 21 and 37 with twelve (27 and 44).
+// One sequence of 16384 x 1024: 44 and 78 us with four, of 52433 x 192: 42 and 73 with sixteen (56 and 105 with eight), of
+// 18285 x 256: 21 and 37 with twelve (27 and 44).  14 of 2899 x 112, 98 units of which 93 clusters of three run at once: 19 and
+// 33 with two, 23 and 37 with three.
 template <int LANES, int VEC, bool GATED, bool BWD>
 int32_t launch_team(fml_ctx* ctx, Params& p) {
   constexpr int SEG = (BWD ? 16 : 32) / VEC, TILE = 8 * (32 / LANES) * SEG;
@@ -575,6 +576,9 @@ int32_t launch_lanes(fml_ctx* ctx, Params& p) {
     // rows of two sectors, as long as two CTAs share a sequence (one of 9000 x 2600 with four lanes 73 and 215 us, with eight
     // 62 and 114; of 6618 x 1472 the other way 35 and 59, 31 and 49)
     if (units(4) <= sms) return launch_team<4, VEC, GATED, BWD>(ctx, p);
+  }
+  if constexpr (VEC == 2) {   // one of 60000 x 50: 25 and 41 us with four lanes, 33 and 60 with eight; of 52433 x 190 49 and 82, 43 and 70
+    if (units(4) * MAX_CLUSTER < 2 * sms) return launch_team<4, VEC, GATED, BWD>(ctx, p);   // rows of one sector
   }
   return launch_team<8, VEC, GATED, BWD>(ctx, p);
 }

@@ -78,7 +78,7 @@ def ctx():
 
 
 class Case:
-    def __init__(self, ctx, n_seq, seq_len, dim, form="gated", layout="sequence", ragged=False, ends=True, seed=0):
+    def __init__(self, ctx, n_seq, seq_len, dim, form="gated", layout="sequence", ragged=False, ends=True, seed=0, lead=1):
         rng = np.random.default_rng(seed + n_seq * 7 + seq_len + dim)
         self.ctx, self.size, self.form, self.layout = ctx, (n_seq, seq_len, dim), form, layout
         self.f = (1.5 * rng.standard_normal((n_seq, seq_len, dim)) + 2).astype(f32)
@@ -88,7 +88,7 @@ class Case:
         self.dy = rng.standard_normal((n_seq, seq_len, dim)).astype(f32)
         self.h0 = rng.standard_normal((n_seq, dim)).astype(f32) if ends else np.zeros((n_seq, dim), f32)
         self.dh_last = rng.standard_normal((n_seq, dim)).astype(f32) if ends else np.zeros((n_seq, dim), f32)
-        self.ends = ends
+        self.ends, self.lead = ends, lead   # lead: floats in front of every array
         self.lens = np.full(n_seq, seq_len)
         if ragged:
             self.lens = rng.integers(0, seq_len + 1, n_seq)
@@ -109,7 +109,7 @@ class Case:
             self.si = self.sh = (seq_len * dim, dim)
             self.apart = n_seq * seq_len * dim
         span = (n_seq - 1) * self.si[0] + (seq_len - 1) * self.si[1] + dim
-        self.n_in, self.n_h = span + self.apart + 2, (n_seq - 1) * self.sh[0] + (seq_len - 1) * self.sh[1] + dim + 2
+        self.n_in, self.n_h = span + self.apart + 1 + self.lead, (n_seq - 1) * self.sh[0] + (seq_len - 1) * self.sh[1] + dim + 1 + self.lead
 
     def index(self, strides, start=0):
         n, t, d = self.size
@@ -122,8 +122,8 @@ class Case:
         return host
 
     def inputs(self):
-        b = self.ctx.upload(self.place(self.n_in, [(self.index(self.si, 1), self.f), (self.index(self.si, 1 + self.apart), self.x)]))
-        return b.view(1, ()), b.view(1 + self.apart, ()), b
+        b = self.ctx.upload(self.place(self.n_in, [(self.index(self.si, self.lead), self.f), (self.index(self.si, self.lead + self.apart), self.x)]))
+        return b.view(self.lead, ()), b.view(self.lead + self.apart, ()), b
 
     def forward(self, h=None, h0=None, last=None):
         from flutter_ml_b200 import ops
@@ -131,19 +131,19 @@ class Case:
         h = h or self.ctx.upload(self.place(self.n_h, []))
         h0 = h0 or (self.ctx.upload(self.h0) if self.ends else None)
         last = last or self.ctx.upload(np.full(self.h0.shape, 7, f32))
-        ops.gated_recurrence_forward(self.ctx, f, x, h.view(1, ()), *self.size, form=self.form, h0=h0, lens=self.dlens, h_last=last,
+        ops.gated_recurrence_forward(self.ctx, f, x, h.view(self.lead, ()), *self.size, form=self.form, h0=h0, lens=self.dlens, h_last=last,
                                      strides_in=self.si, strides_h=self.sh)
         return h, last
 
     def backward(self, h, out=None, dh0=None, accumulate=False, dy=True):
         from flutter_ml_b200 import ops
         f, x, keep = self.inputs()
-        hd = self.ctx.upload(self.place(self.n_h, [(self.index(self.sh, 1), h)]))
-        dyd = self.ctx.upload(self.place(self.n_h, [(self.index(self.sh, 1), self.dy)])) if dy else None
+        hd = self.ctx.upload(self.place(self.n_h, [(self.index(self.sh, self.lead), h)]))
+        dyd = self.ctx.upload(self.place(self.n_h, [(self.index(self.sh, self.lead), self.dy)])) if dy else None
         out = out or self.ctx.upload(self.place(self.n_in, []))
         dh0 = dh0 or self.ctx.upload(np.full(self.h0.shape, 7, f32))
-        ops.gated_recurrence_backward(self.ctx, f, x, hd.view(1, ()), dyd.view(1, ()) if dy else None, out.view(1, ()),
-                                      out.view(1 + self.apart, ()), *self.size, form=self.form, h0=self.ctx.upload(self.h0) if self.ends else None,
+        ops.gated_recurrence_backward(self.ctx, f, x, hd.view(self.lead, ()), dyd.view(self.lead, ()) if dy else None, out.view(self.lead, ()),
+                                      out.view(self.lead + self.apart, ()), *self.size, form=self.form, h0=self.ctx.upload(self.h0) if self.ends else None,
                                       lens=self.dlens, dh_last=self.ctx.upload(self.dh_last) if self.ends else None, dh0=dh0,
                                       strides_in=self.si, strides_h=self.sh, accumulate=accumulate)
         return out, dh0
@@ -158,41 +158,62 @@ SIZES = [(1, 1, 1), (128, 1, 512), (3, 2, 33), (2, 4, 70), (2, 5, 5), (1, 16, 32
          (40, 257, 65), (5, 1000, 64), (3, 2049, 24), (1, 5000, 8), (1, 9001, 1), (1, 4097, 250), (300, 130, 96), (2, 700, 600), (1, 20000, 64), (1, 13000, 130), (40, 60, 130), (50, 40, 33), (3, 150, 1667)]
 
 
-@pytest.mark.gpu
-@pytest.mark.parametrize("form", ["gated", "linear"])
-@pytest.mark.parametrize("layout,ragged", [("sequence", False), ("sequence", True), ("time", True), ("fused", True), ("padded", False)])
-@pytest.mark.parametrize("size", SIZES, ids=str)
-def test_forward_and_backward(ctx, size, layout, ragged, form):
-    c = Case(ctx, *size, form=form, layout=layout, ragged=ragged, ends=layout != "fused")
+def both_directions(ctx, size, layout, ragged, form, lead):
+    c = Case(ctx, *size, form=form, layout=layout, ragged=ragged, ends=layout != "fused", lead=lead)
     there = (np.arange(size[1])[None, :] < c.lens[:, None])[..., None] & np.ones(size, bool)
     ref, bound, last, blast = forward64(c.f, c.x, c.h0, c.lens, form)
     h, end = c.forward()
     flat = h.numpy()
-    got = flat[c.index(c.sh, 1)]
+    got = flat[c.index(c.sh, lead)]
     close(np.where(there, got, 0), np.where(there, ref, 0), bound, "h")
     assert (got[~there] == 7).all()                                      # rows behind the ends, and all around
     around = np.ones(c.n_h, bool)
-    around[c.index(c.sh, 1)] = False
+    around[c.index(c.sh, lead)] = False
     assert (flat[around] == 7).all()
     close(end.numpy(), last, blast, "h_last")
     given = np.where(there, ref, 0).astype(f32)
     rf, rx, r0 = backward64(c.f, c.x, c.h0, given, c.dy, c.dh_last, c.lens, form)
     out, dh0 = c.backward(given)
     flat = out.numpy()
-    for start, (r, b), what in ((1, rf, "df"), (1 + c.apart, rx, "dx")):
+    for start, (r, b), what in ((lead, rf, "df"), (lead + c.apart, rx, "dx")):
         got = flat[c.index(c.si, start)]
         close(np.where(there, got, 0), r, b, what)
         assert (got[~there] == 7).all()
     around = np.ones(c.n_in, bool)
-    around[c.index(c.si, 1)] = around[c.index(c.si, 1 + c.apart)] = False
+    around[c.index(c.si, lead)] = around[c.index(c.si, lead + c.apart)] = False
     assert (flat[around] == 7).all()
     close(dh0.numpy(), *r0, "dh0")
     again, dh0b = c.backward(given, ctx.upload(np.full(c.n_in, 2, f32)), ctx.upload(np.full(c.h0.shape, 2, f32)), accumulate=True)
     flat2 = again.numpy()
-    for start in (1, 1 + c.apart):
+    for start in (lead, lead + c.apart):
         i = c.index(c.si, start)
         assert np.array_equal(flat2[i], np.where(there, flat[i] + f32(2), f32(2)))
     assert np.array_equal(dh0b.numpy(), dh0.numpy() + f32(2))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["gated", "linear"])
+@pytest.mark.parametrize("layout,ragged", [("sequence", False), ("sequence", True), ("time", True), ("fused", True), ("padded", False)])
+@pytest.mark.parametrize("size", SIZES, ids=str)
+def test_forward_and_backward(ctx, size, layout, ragged, form):
+    both_directions(ctx, size, layout, ragged, form, 1)
+
+
+# Addresses that let a lane take two or four channels at once, and among the sizes one for every way of sharing out the
+# channels: many and few sequences, few and many channels, one CTA for all steps or clusters of them.
+WIDE = [(4, s) for s in [(5, 3, 64), (150, 20, 512), (160, 20, 192), (8, 600, 1000), (75, 300, 64), (1, 5000, 64), (2, 2000, 192),
+                         (1, 9001, 256), (1, 700, 2600), (3, 129, 20)]]
+WIDE += [(2, s) for s in [(5, 4, 66), (300, 20, 130), (160, 20, 98), (8, 300, 1022), (50, 100, 50), (40, 300, 62), (1, 3000, 18),
+                          (2, 2000, 250), (1, 2500, 1350), (3, 150, 64)]]
+WIDE += [(1, (40, 300, 33))]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["gated", "linear"])
+@pytest.mark.parametrize("layout,ragged", [("sequence", False), ("time", True), ("fused", True)])
+@pytest.mark.parametrize("lead,size", WIDE, ids=str)
+def test_wide_loads(ctx, lead, size, layout, ragged, form):
+    both_directions(ctx, size, layout, ragged, form, lead)
 
 
 @pytest.mark.gpu
