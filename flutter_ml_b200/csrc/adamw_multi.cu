@@ -26,7 +26,7 @@
 // The moments are formed with one rounding an operation (no contraction), so a restatement in any IEEE float32 arithmetic
 // reproduces the codes bit for bit, but for a root that is one unit off (see roots8) at the border of two codes.
 //
-// Measured on 141 M parameters: 32 bits 566 us, 7.0 TB/s; 8 bits 356 us in short runs (6.4 TB/s), 395 in long ones, where the
+// Measured on 141 M parameters: 32 bits 566 us, 7.0 TB/s; 8 bits 356 us in short runs (6.4 TB/s), 400 in long ones, where the
 // power cap lowers the clock: about 60 instructions an element, 0.8 of the issue slots.  The first form, codes taken apart by
 // shifts and selections, took 549.  Persistent CTAs with the next block in registers: 460 (two CTAs an SM).
 #include <math.h>
