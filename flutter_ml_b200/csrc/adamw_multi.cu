@@ -24,10 +24,9 @@
 // finite is held as NaN and left out of the block's scale: it damages nothing but itself.
 //
 // The moments are formed with one rounding an operation (no contraction), so a restatement in any IEEE float32 arithmetic
-// reproduces the codes bit for bit, but for a root that is one unit off (see roots8) at the border of two codes.
+// reproduces the codes bit for bit; the root is the rounded one.
 //
-// Measured on 141 M parameters: 32 bits 566 us, 7.0 TB/s; 8 bits 356 us in short runs (6.4 TB/s), 400 in long ones, where the
-// power cap lowers the clock: about 60 instructions an element, 0.8 of the issue slots.  The first form, codes taken apart by
+// Measured on 141 M parameters: 32 bits 566 us, 7.0 TB/s; 8 bits 380 us (6.0 TB/s), bound by instructions.  The first form, codes taken apart by
 // shifts and selections, took 549.  Persistent CTAs with the next block in registers: 460 (two CTAs an SM).
 #include <math.h>
 
@@ -128,30 +127,6 @@ __device__ __forceinline__ uint32_t pack8(const uint32_t* z) {
   return __byte_perm(__byte_perm(z[0], z[1], 0x0073), __byte_perm(z[2], z[3], 0x0073), 0x5410);
 }
 
-// Square roots of eight numbers >= 0, one Newton step on the hardware's reciprocal root (Markstein's form: the residual
-// v - s s is exact, so the result is the rounded root but for about one number in a million, one unit off).  Zeros, the
-// smallest numbers and what is not finite go through the library's root: half of it is the test for them, here made once.
-__device__ __forceinline__ void roots8(const float* v, float* root) {
-  float least = INFINITY, all = 0.f;
-#pragma unroll
-  for (int j = 0; j < 8; j++) {
-    least = fminf(least, v[j]);
-    all += v[j];
-  }
-  if (least >= 0x1p-100f && all < INFINITY) {
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      float y;
-      asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(v[j]));
-      const float s = v[j] * y;
-      root[j] = fmaf(fmaf(-s, s, v[j]), 0.5f * y, s);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; j++) root[j] = __fsqrt_rn(v[j]);
-  }
-}
-
 // A warp's block on its way through the registers: eight elements a lane, 4 l .. 4 l + 3 and 128 + 4 l ..
 template <bool EIGHT>
 struct Block {
@@ -236,10 +211,10 @@ __device__ __forceinline__ void update_block(Block<EIGHT>& k, float* mbuf, float
     vv[j] = __fadd_rn(__fmul_rn(v, h.b2), __fmul_rn(__fmul_rn(gj, gj), h.omb2));
   }
   float root[8], mmax = 0.f, rmax = 0.f, all = 0.f;
-  roots8(vv, root);
 #pragma unroll
   for (int j = 0; j < 8; j++) {
     const float m = mv[j];
+    root[j] = __fsqrt_rn(vv[j]);
     // the hardware's reciprocal, good to one unit in the last place: it moves w by lr times that
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(fmaf(root[j], h.rc2, h.eps)));

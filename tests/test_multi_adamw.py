@@ -466,3 +466,24 @@ def test_optimizer_class_beside_adamw(ctx, bits):
         O.MultiTensorAdamW([], 0.01)
     with pytest.raises(ValueError):
         O.MultiTensorAdamW(a, 0.01, seed=-3)
+
+
+@pytest.mark.gpu
+def test_roots_at_the_borders_of_the_codes(ctx):
+    """Nearest rounding where one unit in the last place of the root changes its code: beta1 = beta2 = 0 make v the rounded
+    square of the gradient, and the gradients are the midpoints between neighbouring codes (and up to six units beside them),
+    a block for each power of two from 2^-55 to 2^55 whose largest element, 448 of it, fixes the scale."""
+    mids = np.array([m * 2.0 ** e for e in range(-2, 8) for m in (1.0625, 1.1875, 1.3125, 1.4375, 1.5625, 1.6875)], f32)
+    blocks = np.concatenate([mids * f32(1 + k * 2.0 ** -23) for k in (0, 1, -1, 6)] + [np.full(16, 448, f32)])   # 256 elements
+    assert blocks.size == 256
+    exps = range(-55, 56)
+    s = Setup(ctx, [256 * len(exps)], 8, seed=1)
+    g = np.concatenate([blocks * f32(2.0 ** e) for e in exps]).astype(f32)
+    ctx.upload(g, out=s.dg.view(s.off[0], (g.size,)))
+    s.plan.step(1e-3, 0.0, 0.0, 1e-8, 0.0, 1, seed=-1)
+    code, scale = to_codes(np.sqrt((g * g).astype(f32)).reshape(-1, 256), None, True)
+    rc, rs = s.states(s.v)[0]
+    assert np.array_equal(rs, scale) and np.array_equal(rc, code)
+    code, scale = to_codes(g.reshape(-1, 256), None, False)
+    mc, ms = s.states(s.m)[0]
+    assert np.array_equal(ms, scale) and np.array_equal(mc, code)
