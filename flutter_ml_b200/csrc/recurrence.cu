@@ -69,9 +69,14 @@ __device__ __forceinline__ void gate(float f, float& a, float& s) {
   }
 }
 
-// "state <- A state + B".  LINEAR decays may be above one: a zero state stays clear of a product of them that has overflowed
+// "state <- A state + B".  GATED decays are positive, and a product of them that has underflowed counts as the smallest number
+// above zero: an infinite state stays infinite, a finite one is off by 2^-149 of itself.  (A gate that is NaN shows in B.)
+// LINEAR ones may be above one: a zero state stays clear of a product of them that has overflowed.
 template <bool GATED>
-__device__ __forceinline__ float through(float A, float B, float state) { return !GATED && state == 0.f ? B : fmaf(A, state, B); }
+__device__ __forceinline__ float through(float A, float B, float state) {
+  if (GATED) return fmaf(fmaxf(A, 0x1p-149f), state, B);
+  return state == 0.f ? B : fmaf(A, state, B);
+}
 
 // A pair into the shared memory of CTA `rank` of the cluster, counted by that CTA's barrier: neither side needs a fence, which
 // would wait for the results of the round before as well (the cluster's own barrier did).

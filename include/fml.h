@@ -561,7 +561,8 @@ int32_t fml_lstm_cell_bwd(fml_ctx* ctx, const float* gates, const float* c_prev,
 /* ---- gated linear recurrence ---------------------------------------------------
  * (Extension beside the LSTM: gates that do not read the state, so the steps can be joined in any grouping.)  For every
  * sequence s, channel c and step t < lens[s] (lens NULL: seq_len), from h0 [n_seq][dim] (NULL: zero):
- *   FML_RECURRENCE_GATED   a = sigmoid(f),  h_t = a h_{t-1} + (1 - a) x_t   (f below -80 counts as -80)
+ *   FML_RECURRENCE_GATED   a = sigmoid(f),  h_t = a h_{t-1} + (1 - a) x_t   (f below -80 counts as -80, so that a is
+ *                          positive and an infinite state stays infinite; above 87 the factor 1 - a is zero)
  *   FML_RECURRENCE_LINEAR  a = f,           h_t = a h_{t-1} + x_t
  * Element (s, t, c) of f and x lies at s * seq_stride_in + t * step_stride_in + c (elements; both arrays share the strides,
  * so they may be the halves of one fused projection), of h at the strides of h: sequence-major, time-major and sliced

@@ -462,3 +462,39 @@ def test_layer_on_the_tape(ctx, output, ragged):
     for bad in (dict(n_seq=2, seq_len=S), dict(n_seq=n, seq_len=S, output="first"), dict(n_seq=n, seq_len=S, lens=ctx.zeros(3))):
         with pytest.raises(ValueError):
             T.gatedRecurrence(T.Tensor(np.zeros((n * S, 2 * H), f32), ctx), **bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["sequence", "fused"])
+@pytest.mark.parametrize("lead,size", [(1, (2, 3, 20)), (1, (2, 300, 20)), (1, (1, 9001, 12)), (4, (1, 5000, 64)), (4, (1, 9001, 256)), (2, (1, 6000, 18)),
+                                       (4, (160, 2000, 64)), (4, (75, 3000, 64))], ids=str)
+def test_an_infinite_state_stays_infinite(ctx, lead, size, layout):
+    """GATED: all gates are positive, so a state that has become infinite stays so through any number of them, also where
+    their product is far below float32's range; likewise an infinite gradient on its way back."""
+    n, seq_len, _ = size
+    c = Case(ctx, *size, layout=layout, lead=lead)
+    clean = c.forward()[0].numpy()[c.index(c.sh, lead)]
+    t, s = seq_len // 3, n - 1
+    c.x[s, t, 3], c.x[s, t, 4], c.h0[s, 5] = np.inf, -np.inf, np.inf
+    h, last = c.forward()
+    h, last = h.numpy()[c.index(c.sh, lead)], last.numpy()
+    assert (h[s, t:, 3] == np.inf).all() and (h[s, t:, 4] == -np.inf).all() and (h[s, :, 5] == np.inf).all()
+    assert last[s, 3] == np.inf and last[s, 4] == -np.inf and last[s, 5] == np.inf
+    assert np.array_equal(h[s, :t, 3:5], clean[s, :t, 3:5])
+    rest = np.ones(size, bool)
+    rest[s, :, 3:6] = False
+    assert np.array_equal(h[rest], clean[rest])
+    c.x[s, t, 3:5], c.h0[s, 5] = 0, 0
+    given = forward64(c.f, c.x, c.h0, c.lens, "gated")[0].astype(f32) if seq_len < 4000 else clean
+    clean, clean0 = (v.numpy() for v in c.backward(given))
+    clean = [clean[c.index(c.si, lead + o)] for o in (0, c.apart)]
+    c.dy[s, t, 3], c.dy[s, t, 4], c.dh_last[s, 5] = np.inf, -np.inf, np.inf
+    out, dh0 = (v.numpy() for v in c.backward(given))
+    df, dx = out[c.index(c.si, lead)], out[c.index(c.si, lead + c.apart)]
+    assert (dx[s, :t + 1, 3] == np.inf).all() and (dx[s, :t + 1, 4] == -np.inf).all() and (dx[s, :, 5] == np.inf).all()
+    assert np.array_equal(dh0[s, 3:6], np.array([np.inf, -np.inf, np.inf], f32))
+    assert np.isinf(df[s, :t + 1, 3:5]).all() and np.isinf(df[s, :, 5]).all()
+    for got, want in ((df, clean[0]), (dx, clean[1])):
+        assert np.array_equal(got[s, t + 1:, 3:5], want[s, t + 1:, 3:5]) and np.array_equal(got[rest], want[rest])
+    rest0 = rest[:, 0]
+    assert np.array_equal(dh0[rest0], clean0[rest0])
