@@ -569,8 +569,9 @@ int32_t fml_lstm_cell_bwd(fml_ctx* ctx, const float* gates, const float* c_prev,
  * layouts alike.  h_last [n_seq][dim] (or NULL) receives the state after each sequence's last step and may be h0 itself.
  * Rows of h behind a sequence's end are left as they were.  A length outside [0, seq_len] (device memory) is reported by
  * fml_device_status and taken as the nearest of the two.  One step at a time is the same call with seq_len = 1.
- * LINEAR: the decays of up to 2048 neighbouring steps are multiplied in float32; where such a product leaves float32's
- * range while the states do not, the result is the one with the product at infinity or zero.
+ * LINEAR: the decays of up to 1024 neighbouring steps are multiplied in float32.  Where the product of some run of them is
+ * below float32's range, nothing of a finite state before the run is left; where one is above it (decays above one)
+ * although the states are not, states from there on may be infinite or NaN.
  * Backward, from the forward call's inputs and its h: dy (strides of h; NULL: zero) and dh_last (NULL: zero) are the
  * gradients of h and h_last; df and dx (strides of f and x) and dh0 (NULL: not wanted) are overwritten, or added to when
  * accumulate != 0; rows behind a sequence's end are left as they were.  dh0 may be dh_last itself when nothing is added.
