@@ -291,7 +291,8 @@ __device__ __forceinline__ void update_block(Block<EIGHT>& k, float* mbuf, float
     if (odd) {
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        if (!finite_bits(__float_as_uint(mv[4 * q + i]))) mo[q] |= 0xffu << (8 * i);
+        const uint32_t b = __float_as_uint(mv[4 * q + i]);
+        if (!finite_bits(b)) mo[q] = (mo[q] & ~(0xffu << (8 * i))) | (b == 0xff800000u ? 0xffu : 0x7fu) << (8 * i);
         if (!finite_bits(__float_as_uint(root[4 * q + i]))) ro[q] = (ro[q] & ~(0xffu << (8 * i))) | 0x7fu << (8 * i);
       }
     }

@@ -348,8 +348,9 @@ int32_t fml_optimizer_step(fml_ctx* ctx, int32_t kind, float* w, const float* g,
  *   m, v         one buffer each for the whole list, 16-byte aligned, of fml_adamw_state_floats floats, zeroed before the
  *                first step.  Tensor i owns the blocks of 256 elements that follow those of tensor i - 1 (its last block may
  *                be partly unused).  32 bits: m and v, 256 floats a block.  8 bits: first the codes of all blocks, 256
- *                bytes each (sign, 4 exponent and 3 fraction bits, 0x7f NaN), then one float32 scale, a power of two, for
- *                each block; an element is code * scale, and the second buffer holds sqrt(v).
+ *                bytes each (sign, 4 exponent and 3 fraction bits; 0x7f is NaN and stands for what is not finite, 0xff
+ *                for minus infinity), then one float32 scale, a power of two, for each block; an element is code * scale,
+ *                and the second buffer holds sqrt(v).
  * Steps of one plan follow each other (they update the same buffers); different plans may run at once on different lanes.
  * A plan belongs to its context, which frees those that are left at fml_shutdown; it must outlive the graphs that were
  * recorded with it.  Make and destroy plans outside recordings (both wait for the device). */

@@ -487,3 +487,23 @@ def test_roots_at_the_borders_of_the_codes(ctx):
     code, scale = to_codes(g.reshape(-1, 256), None, False)
     mc, ms = s.states(s.m)[0]
     assert np.array_equal(ms, scale) and np.array_equal(mc, code)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seed", [-1, 4])
+def test_codes_of_values_that_are_not_finite(ctx, seed):
+    """NaN and both infinities among ordinary gradients, and a square that overflows: the codes are the restatement's."""
+    s = Setup(ctx, [1024], 8, seed=2)
+    g = s.tensors(s.g)[0]
+    g[[5, 300, 301, 700, 1023]] = np.nan, np.inf, -np.inf, -np.inf, 3e38
+    ctx.upload(g, out=s.dg.view(s.off[0], (1024,)))
+    s.step(1, seed=seed)
+    with np.errstate(over="ignore"):
+        m, v = moments32(np.zeros((4, 256), f32), np.zeros((4, 256), f32), g.reshape(4, 256), 0.9, 0.999)
+    m[np.isnan(m)] = np.nan             # the sign of a NaN is the processor's choice
+    rnd = words(4, seed, 1) if seed >= 0 else None
+    for (got, sc), x, half, root in ((s.states(s.m)[0], m, 16, False), (s.states(s.v)[0], np.sqrt(v), 0, True)):
+        code, scale = to_codes(x, None if rnd is None else (rnd >> half) & 0xFFFF, root)
+        assert np.array_equal(got, code) and np.array_equal(sc, scale)
+    mc = s.states(s.m)[0][0].reshape(-1)
+    assert list(mc[[5, 300, 301, 700]]) == [0x7f, 0x7f, 0xff, 0xff]
