@@ -420,6 +420,12 @@ class FmlBindings {
   late final fmlAdamwPlanStep = lib.lookupFunction<
       Int32 Function(Pointer<FmlCtx>, Int32, Int32, Double, Double, Double, Double, Double, Int32, Double, Int32, Int64),
       int Function(Pointer<FmlCtx>, int, int, double, double, double, double, double, int, double, int, int)>('fml_adamw_plan_step');
+  late final fmlAdamwPlanCount = lib.lookupFunction<
+      Int32 Function(Pointer<FmlCtx>, Int32, Pointer<Int32>),
+      int Function(Pointer<FmlCtx>, int, Pointer<Int32>)>('fml_adamw_plan_count');
+  late final fmlAdamwPlanSetCount = lib.lookupFunction<
+      Int32 Function(Pointer<FmlCtx>, Int32, Int32),
+      int Function(Pointer<FmlCtx>, int, int)>('fml_adamw_plan_set_count');
   late final fmlAdamwPlanDestroy = lib.lookupFunction<
       Int32 Function(Pointer<FmlCtx>, Int32),
       int Function(Pointer<FmlCtx>, int)>('fml_adamw_plan_destroy');

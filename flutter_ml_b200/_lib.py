@@ -138,6 +138,8 @@ PROTOTYPES = {
     "fml_adamw_state_floats": [i32, fp, i32, C.POINTER(i64)],
     "fml_adamw_plan_create": [fp, i32, fp, fp, fp, fp, fp, i32, C.POINTER(i32)],
     "fml_adamw_plan_step": [fp, i32, i32, C.c_double, C.c_double, C.c_double, C.c_double, C.c_double, i32, C.c_double, i32, i64],
+    "fml_adamw_plan_count": [fp, i32, C.POINTER(i32)],
+    "fml_adamw_plan_set_count": [fp, i32, i32],
     "fml_adamw_plan_destroy": [fp, i32],
     "fml_act2_fwd": [fp, i32, f32, fp, fp, i64],
     "fml_act2_bwd": [fp, i32, f32, fp, fp, fp, i64, i32],

@@ -460,6 +460,28 @@ int32_t fml_adamw_plan_step(fml_ctx* ctx, int32_t plan_id, int32_t lane, double 
   return FML_OK;
 }
 
+// The plan's own counter, once every step enqueued so far has run, on whatever stream
+static int32_t counter(fml_ctx* ctx, int32_t plan_id, int* t, bool set) {
+  FML_ENTER(ctx);
+  FML_REQUIRE(ctx, plan_id >= 0 && plan_id < (int32_t)ctx->adamw_plans.size() && ctx->adamw_plans[plan_id], "fml_adamw_plan_count: unknown plan");
+  FML_REQUIRE(ctx, !ctx->capturing, "fml_adamw_plan_count: not while a graph is being recorded");
+  FML_CUDA(ctx, cudaDeviceSynchronize());
+  int* at = &ctx->adamw_plans[plan_id]->step->t;
+  FML_CUDA(ctx, set ? cudaMemcpy(at, t, sizeof(int), cudaMemcpyHostToDevice) : cudaMemcpy(t, at, sizeof(int), cudaMemcpyDeviceToHost));
+  if (set) FML_CUDA(ctx, cudaDeviceSynchronize());
+  return FML_OK;
+}
+
+int32_t fml_adamw_plan_count(fml_ctx* ctx, int32_t plan_id, int32_t* t) {
+  FML_REQUIRE(ctx, ctx && t, "fml_adamw_plan_count: bad arguments");
+  return counter(ctx, plan_id, t, false);
+}
+
+int32_t fml_adamw_plan_set_count(fml_ctx* ctx, int32_t plan_id, int32_t t) {
+  FML_REQUIRE(ctx, ctx && t >= 0, "fml_adamw_plan_set_count: the number of steps must not be negative");
+  return counter(ctx, plan_id, &t, true);
+}
+
 int32_t fml_adamw_plan_destroy(fml_ctx* ctx, int32_t plan_id) {
   FML_REQUIRE(ctx, ctx, "fml_adamw_plan_destroy: no context");
   FML_ENTER(ctx);

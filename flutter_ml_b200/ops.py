@@ -282,6 +282,17 @@ class AdamWPlan:
                                                         1 if zero_grad else 0, seed))
         self.ctx.launches += 1 if t else 2
 
+    @property
+    def count(self) -> int:
+        """Steps counted on the device so far (those with t = 0); setting it goes on from a checkpoint."""
+        t = ctypes.c_int32(0)
+        self.ctx.check(self.ctx.lib.fml_adamw_plan_count(self.ctx.h, self.id, ctypes.byref(t)))
+        return t.value
+
+    @count.setter
+    def count(self, t: int):
+        self.ctx.check(self.ctx.lib.fml_adamw_plan_set_count(self.ctx.h, self.id, t))
+
     def close(self):
         if self.id >= 0 and self.ctx.h:
             self.ctx.check(self.ctx.lib.fml_adamw_plan_destroy(self.ctx.h, self.id))

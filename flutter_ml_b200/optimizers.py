@@ -219,7 +219,8 @@ class MultiTensorAdamW(Optimizer):
     stateBits=8 rounds the moments at random by `seed` (the same seed repeats a run exactly) unless `seed` is None, which
     rounds to the nearest code.  Gradients that do not exist yet are created, zeroed, here.  `step()` looks at the tensors'
     and gradients' addresses and makes its plan anew where one has changed.  deviceCounter=True keeps the step count on the
-    device, so that a recorded step (`graph_begin`) advances it at every replay."""
+    device, so that a recorded step (`graph_begin`) advances it at every replay; `checkpoint.save_training_state` and
+    `load_training_state` read and set it there."""
 
     def __init__(self, parameters, learningRate, beta1=0.9, beta2=0.999, epsilon=1e-8, weightDecay=0.01, stateBits=32,
                  seed: Optional[int] = 0, deviceCounter: bool = False):
@@ -229,7 +230,7 @@ class MultiTensorAdamW(Optimizer):
         if seed is not None and seed < 0:
             raise ValueError("MultiTensorAdamW: seed must not be negative (None rounds to the nearest)")
         self.beta1, self.beta2, self.epsilon, self.weightDecay = beta1, beta2, epsilon, weightDecay
-        self.stateBits, self.seed, self.deviceCounter, self._t = stateBits, seed, deviceCounter, 0
+        self.stateBits, self.seed, self.deviceCounter, self._steps = stateBits, seed, deviceCounter, 0
         self.ctx = self.parameters[0].ctx
         self._sizes = [p.value.size for p in self.parameters]
         n = AdamWPlan.state_floats(self._sizes, stateBits)
@@ -239,6 +240,17 @@ class MultiTensorAdamW(Optimizer):
                 p.zeroGrad()
         self._plan, self._at = None, None
         self._current_plan()
+
+    @property
+    def _t(self) -> int:
+        return self._plan.count if self.deviceCounter else self._steps
+
+    @_t.setter
+    def _t(self, t: int):
+        if self.deviceCounter:
+            self._plan.count = t
+        else:
+            self._steps = t
 
     def _current_plan(self):
         if any(p.grad is None for p in self.parameters):
@@ -257,6 +269,7 @@ class MultiTensorAdamW(Optimizer):
 
     def step(self, grad_scale: float = 1.0, zero_grad: bool = False):
         plan = self._current_plan()
-        self._t += 1
-        plan.step(self.learningRate, self.beta1, self.beta2, self.epsilon, self.weightDecay, 0 if self.deviceCounter else self._t,
+        if not self.deviceCounter:
+            self._steps += 1
+        plan.step(self.learningRate, self.beta1, self.beta2, self.epsilon, self.weightDecay, 0 if self.deviceCounter else self._steps,
                   grad_scale, zero_grad, -1 if self.seed is None else self.seed)

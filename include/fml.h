@@ -364,6 +364,10 @@ int32_t fml_adamw_plan_create(fml_ctx* ctx, int32_t n, float* const* w, float* c
  * over (seed, t, block, element) - the same call gives the same bits.  eps must be 1e-37 or more, betas in [0, 1). */
 int32_t fml_adamw_plan_step(fml_ctx* ctx, int32_t plan_id, int32_t lane, double lr, double beta1, double beta2, double eps,
                             double weight_decay, int32_t t, double grad_scale, int32_t zero_grad, int64_t seed);
+/* The number of steps with t = 0 so far (a new plan: 0), for a checkpoint, and setting it, to go on from one.  Both wait
+ * for the device; not while a graph is being recorded. */
+int32_t fml_adamw_plan_count(fml_ctx* ctx, int32_t plan_id, int32_t* t);
+int32_t fml_adamw_plan_set_count(fml_ctx* ctx, int32_t plan_id, int32_t t);
 int32_t fml_adamw_plan_destroy(fml_ctx* ctx, int32_t plan_id);
 
 /* The other activations of lib/activationFunctions, with their parameter: FML_ACT2_LEAKY_RELU (alpha, leakyRelu.dart:35-48),

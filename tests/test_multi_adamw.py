@@ -507,3 +507,53 @@ def test_codes_of_values_that_are_not_finite(ctx, seed):
         assert np.array_equal(got, code) and np.array_equal(sc, scale)
     mc = s.states(s.m)[0][0].reshape(-1)
     assert list(mc[[5, 300, 301, 700]]) == [0x7f, 0x7f, 0xff, 0xff]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("device", [True, False])
+def test_training_goes_on_from_a_checkpoint(ctx, tmp_path, bits, device):
+    """Three steps, a checkpoint, two more; an optimizer that loads the checkpoint takes the same two, bit for bit.  With the
+    count on the device the steps are replays of a recording, which the host does not count."""
+    from flutter_ml_b200 import checkpoint, optimizers as O
+    from flutter_ml_b200.tensor import Tensor
+    rng = np.random.default_rng(3)
+    shapes, path = [(40, 50), (7,)], str(tmp_path / "state")
+    init, grads = ([rng.standard_normal(s).astype(f32) for s in shapes] for _ in range(2))
+
+    def start(values):
+        ps = [Tensor(x, ctx) for x in values]
+        for p, g in zip(ps, grads):
+            p.grad = ctx.upload(g)
+        return ps, O.MultiTensorAdamW(ps, 0.01, stateBits=bits, seed=5, deviceCounter=device)
+
+    def run(opt, steps):
+        if not device:
+            for _ in range(steps):
+                opt.step()
+            return
+        ctx.sync()
+        ctx.graph_begin()
+        opt.step()
+        gid = ctx.graph_end()
+        for _ in range(steps):
+            ctx.graph_launch(gid)
+        ctx.sync()
+        ctx.check(ctx.lib.fml_graph_destroy(ctx.h, gid))
+    a, oa = start(init)
+    run(oa, 3)
+    assert oa._t == 3
+    checkpoint.save_training_state(ctx, path, oa)
+    b, ob = start([np.zeros(s, f32) for s in shapes])
+    checkpoint.load_training_state(ctx, path, ob)
+    assert ob._t == 3
+    for o in (oa, ob):
+        run(o, 2)
+        assert o._t == 5
+    for p, q in zip([x.value for x in a] + [oa._m, oa._v], [x.value for x in b] + [ob._m, ob._v]):
+        assert np.array_equal(p.numpy().view(np.int32), q.numpy().view(np.int32))
+    with pytest.raises(Exception, match="negative"):
+        oa._plan.count = -1
+    oa._plan.close()
+    with pytest.raises(Exception, match="unknown plan"):
+        oa._plan.count
