@@ -310,8 +310,7 @@ __device__ __forceinline__ void update_block(Block<EIGHT>& k, float* mbuf, float
 // One work item a CTA: the loads of the other CTAs of the SM run beside its arithmetic.
 template <bool EIGHT, bool NEAREST, bool ZERO>
 __global__ void __launch_bounds__(32 * WARPS, EIGHT ? 5 : 1)
-adamw_kernel(const Item* __restrict__ items, float* __restrict__ mbuf, float* __restrict__ vbuf, long long n_blocks, Hyper h,
-             const DeviceStep* __restrict__ dev) {
+adamw_kernel(const Item* __restrict__ items, float* mbuf, float* vbuf, long long n_blocks, Hyper h, const DeviceStep* dev) {
   fml_chain_next();
   const Item it = items[blockIdx.x];                  // the plan's own table: written before any step
   fml_chain_wait();

@@ -102,7 +102,9 @@ int32_t fml_ensure_workspace_keep(fml_ctx* ctx, size_t bytes);
 
 // Launches a kernel that may be set up while the kernel before it on the stream drains (programmatic dependent launch).  Such
 // a kernel calls fml_chain_next() at its start, so that the one behind it can do the same, and fml_chain_wait() before it
-// touches global memory: that returns when everything before it has finished and is visible.
+// touches global memory: that returns when everything before it has finished and is visible.  The kernel before may still write
+// while this one runs, so memory that it can write is read by plain loads: not by __ldg, and not through __restrict__ pointers,
+// whose loads may go through the read-only path or be moved up across the wait.
 template <class... K, class... A>
 inline cudaError_t fml_launch_chained(void (*kernel)(K...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) {
   cudaLaunchConfig_t cfg = {};

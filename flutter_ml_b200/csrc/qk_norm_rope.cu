@@ -176,7 +176,7 @@ __device__ __forceinline__ void side_heads(const Params& p, const Side& s, const
   float* o0 = s.out + r0 * s.ldo;
   float gain[8];
 #pragma unroll
-  for (int i = 0; i < 8; i++) gain[i] = at.active && s.gain ? __ldg(s.gain + (i < 4 ? at.e0 : at.e1) + (i & 3)) : 1.f;
+  for (int i = 0; i < 8; i++) gain[i] = at.active && s.gain ? s.gain[(i < 4 ? at.e0 : at.e1) + (i & 3)] : 1.f;
   if (start >= total && then) load_item<LPH, BWD>(p, *then, r0, n, start, at, ahead);
   for (int it = start; it < total; it += STEP) {
     Item<BWD> v = ahead;
@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(THREADS) qk_pair_kernel(const Params p) {
 
 // dgain += the CTAs' sums, 32 columns a block, in a fixed order.  32 warps, so that a thread's loads are one trip to memory:
 // with eight it took 10 us.
-__global__ void __launch_bounds__(1024) qk_gain_kernel(const float* __restrict__ parts, int n_parts, int d, float* dgain_q, float* dgain_k) {
+__global__ void __launch_bounds__(1024) qk_gain_kernel(const float* parts, int n_parts, int d, float* dgain_q, float* dgain_k) {
   __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
   fml_chain_next();
