@@ -462,6 +462,11 @@ int32_t check(fml_ctx* ctx, const Params& p, int32_t form) {
   FML_REQUIRE(ctx, p.n_seq >= 0 && p.seq_len >= 0 && p.seq_len <= (1 << 30) && p.dim >= 1, "fml_gated_recurrence: bad sizes");
   FML_REQUIRE(ctx, (long long)p.n_seq * ((p.dim + 7) / 8) <= (1ll << 27), "fml_gated_recurrence: too many sequences and channels for one call");
   FML_REQUIRE(ctx, p.ss_in >= 0 && p.ts_in >= 0 && p.ss_h >= 0 && p.ts_h >= 0, "fml_gated_recurrence: strides must not be negative");
+  uintptr_t all = 0;
+  for (const void* q : {(const void*)p.f, (const void*)p.x, (const void*)p.h0, (const void*)p.lens, (const void*)p.out, (const void*)p.last, (const void*)p.h,
+                        (const void*)p.dy, (const void*)p.dh_last, (const void*)p.df, (const void*)p.dx, (const void*)p.dh0})
+    all |= reinterpret_cast<uintptr_t>(q);
+  FML_REQUIRE(ctx, (all & 3) == 0, "fml_gated_recurrence: misaligned buffer");
   return FML_OK;
 }
 

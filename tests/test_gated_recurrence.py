@@ -498,3 +498,23 @@ def test_an_infinite_state_stays_infinite(ctx, lead, size, layout):
         assert np.array_equal(got[s, t + 1:, 3:5], want[s, t + 1:, 3:5]) and np.array_equal(got[rest], want[rest])
     rest0 = rest[:, 0]
     assert np.array_equal(dh0[rest0], clean0[rest0])
+
+
+@pytest.mark.gpu
+def test_misaligned_addresses_are_refused(ctx):
+    """An address that is no multiple of four bytes would fault in the kernels; each buffer of both calls, one after the other."""
+    import ctypes
+    b = ctx.zeros(4096)
+    at = lambda o: ctypes.c_void_p(b.ptr + 4 * o)  # noqa: E731
+    off = lambda v, k: ctypes.c_void_p(v.value + k)  # noqa: E731
+    fwd = [0, 2, 3, 8, at(0), at(100), 24, 8, at(200), at(300), at(400), 24, 8, at(500)]
+    bwd = [0, 2, 3, 8, at(0), at(100), 24, 8, at(200), at(300), at(400), at(500), 24, 8, at(600), at(700), at(800), at(900), 0]
+    for name, args in (("fml_gated_recurrence_fwd", fwd), ("fml_gated_recurrence_bwd", bwd)):
+        call = lambda a: getattr(ctx.lib, name)(ctx.h, *a)  # noqa: E731
+        assert call(args) == 0
+        for i, v in enumerate(args):
+            if isinstance(v, ctypes.c_void_p):
+                for k in (1, 2):
+                    assert call(args[:i] + [off(v, k)] + args[i + 1:]) != 0, (name, i)
+                    assert b"misaligned" in ctx.lib.fml_last_error(ctx.h)
+    ctx.sync()
