@@ -446,6 +446,8 @@ int32_t check(fml_ctx* ctx, const Params& p, double base) {
   FML_REQUIRE(ctx, p.rot == 0 || (base > 0 && isfinite(base)), "fml_qk_norm_rope: base must be positive");
   FML_REQUIRE(ctx, p.eps >= 1e-37f && isfinite(p.eps), "fml_qk_norm_rope: eps must be 1e-37 or more");
   FML_REQUIRE(ctx, p.seq_len >= 0, "fml_qk_norm_rope: bad seq_len");
+  FML_REQUIRE(ctx, ((reinterpret_cast<uintptr_t>(p.s[0].gain) | reinterpret_cast<uintptr_t>(p.s[1].gain) | reinterpret_cast<uintptr_t>(p.pos)) & 3) == 0,
+              "fml_qk_norm_rope: misaligned gains or positions");
   for (int t = 0; t < 2; t++) {
     const Side& s = p.s[t];
     if (s.heads == 0) continue;
@@ -549,6 +551,8 @@ int32_t fml_qk_norm_rope_bwd(fml_ctx* ctx, const float* q, int64_t ld_q, const f
   FML_REQUIRE(ctx, dq_out && (heads_k == 0 || dk_out), "fml_qk_norm_rope_bwd: missing gradient");
   FML_REQUIRE(ctx, (!dgain_q || gain_q) && (!dgain_k || (gain_k && heads_k)), "fml_qk_norm_rope_bwd: the gradient of a gain that is not there");
   FML_REQUIRE(ctx, !(dgain_q || dgain_k) || scratch, "fml_qk_norm_rope_bwd: gain gradients need the scratch buffer");
+  FML_REQUIRE(ctx, ((reinterpret_cast<uintptr_t>(dgain_q) | reinterpret_cast<uintptr_t>(dgain_k) | reinterpret_cast<uintptr_t>(scratch)) & 3) == 0,
+              "fml_qk_norm_rope_bwd: misaligned gain gradients or scratch buffer");
   const long long sw = (long long)MAX_PARTS * 2 * d_head;
   FML_REQUIRE(ctx, !clash(dgain_q, d_head, d_head, dgain_k, d_head, d_head, 1) && !clash(dgain_q, d_head, d_head, scratch, sw, sw, 1) &&
                        !clash(dgain_k, d_head, d_head, scratch, sw, sw, 1),

@@ -465,3 +465,25 @@ def test_tape_node_leaves_the_values_out(ctx):
     assert np.array_equal(grads[0][1], grads[1][1])
     with pytest.raises(ValueError):
         T.qkNormRope(T.Tensor(x0, ctx), 3, 1, 32)
+
+
+@pytest.mark.gpu
+def test_misaligned_addresses_are_refused(ctx):
+    """An address that is no multiple of four bytes would fault in the kernels; each buffer of both calls, one after the other."""
+    import ctypes
+    from flutter_ml_b200 import _lib
+    d, rows = 64, 8
+    b, s = ctx.zeros(8192), ctx.zeros(_lib.QK_NORM_ROPE_PARTS * 2 * d + 4)
+    at = lambda o: ctypes.c_void_p(b.ptr + 4 * o)  # noqa: E731
+    gq, gk, dgq, dgk, pos, scratch = at(7000), at(7064), at(7128), at(7192), at(7256), ctypes.c_void_p(s.ptr)
+    fwd = [at(0), d, at(512), d, 1, at(1024), d, at(1536), d, 1, rows, d, gq, gk, pos, 0, d, 0, 10000.0, 1e-6]
+    bwd = [at(0), d, at(512), d, at(1024), d, 1, at(1536), d, at(2048), d, at(2560), d, 1, rows, d, gq, gk, dgq, dgk, pos, 0, d, 0, 10000.0, 1e-6, 0, scratch]
+    for name, args in (("fml_qk_norm_rope_fwd", fwd), ("fml_qk_norm_rope_bwd", bwd)):
+        call = lambda a: getattr(ctx.lib, name)(ctx.h, *a)  # noqa: E731
+        assert call(args) == 0
+        for i, v in enumerate(args):
+            if isinstance(v, ctypes.c_void_p):
+                for k in (1, 2):
+                    assert call(args[:i] + [ctypes.c_void_p(v.value + k)] + args[i + 1:]) != 0, (name, i)
+                    assert b"misaligned" in ctx.lib.fml_last_error(ctx.h)
+    ctx.sync()
