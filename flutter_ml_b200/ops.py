@@ -176,8 +176,8 @@ class DenseFwdBwdHost:
 
 
 def _index_buffer(a, n, what):
-    """An int32 buffer of at least n entries, or None; a view without a shape is an address and has no length to check."""
-    if a is not None and (a.dtype != np.int32 or (a.shape != () and a.size < n)):
+    """An int32 buffer of at least n entries; a view without a shape is an address and has no length to check."""
+    if a.dtype != np.int32 or (a.shape and a.size < n):
         raise ValueError(f"{what} must be int32, {n} of them")
 
 
@@ -185,7 +185,8 @@ def gated_recurrence_forward(ctx, f, x, h, n_seq, seq_len, dim, form="gated", h0
     """h_t = a_t h_{t-1} + (1 - a_t) x_t with a = sigmoid(f) (form "gated"), or h_t = f_t h_{t-1} + x_t ("linear"), along every
     sequence (`fml_gated_recurrence_fwd`).  strides_in (f and x) and strides_h are (sequence, step) strides in elements,
     sequence-major without gaps by default; lens: int32 lengths on the device."""
-    _index_buffer(lens, n_seq, "gated_recurrence: lens")
+    if lens is not None:
+        _index_buffer(lens, n_seq, "gated_recurrence: lens")
     dense = (seq_len * dim, dim)
     si, sh = strides_in or dense, strides_h or dense
     rc = ctx.lib.fml_gated_recurrence_fwd(ctx.h, _lib.RECURRENCE_BY_NAME[form], n_seq, seq_len, dim, f and f.ptr, x and x.ptr, si[0], si[1],
@@ -199,7 +200,8 @@ def gated_recurrence_backward(ctx, f, x, h, dy, df, dx, n_seq, seq_len, dim, for
                               strides_in=None, strides_h=None, accumulate=False):
     """Gradients of `gated_recurrence_forward` from its inputs and its h (`fml_gated_recurrence_bwd`); dy may be None (zero),
     df and dx lie at the strides of f and x, dy at those of h."""
-    _index_buffer(lens, n_seq, "gated_recurrence: lens")
+    if lens is not None:
+        _index_buffer(lens, n_seq, "gated_recurrence: lens")
     dense = (seq_len * dim, dim)
     si, sh = strides_in or dense, strides_h or dense
     rc = ctx.lib.fml_gated_recurrence_bwd(ctx.h, _lib.RECURRENCE_BY_NAME[form], n_seq, seq_len, dim, f and f.ptr, x and x.ptr, si[0], si[1],
@@ -219,7 +221,8 @@ def qk_norm_rope_forward(ctx, q, k, q_out, k_out, rows, heads_q, heads_k, d_head
                          rot_dim=None, interleaved=False, base=10000.0, eps=1e-6, ld_q=None, ld_k=None, ld_q_out=None, ld_k_out=None):
     """Norm of every query and key head, its gain, and the rotation by position, in one launch (`fml_qk_norm_rope_fwd`).
     Row strides default to rows that lie end to end; rot_dim defaults to the whole head; k may be None with heads_k = 0."""
-    _index_buffer(positions, rows, "qk_norm_rope: positions")
+    if positions is not None:
+        _index_buffer(positions, rows, "qk_norm_rope: positions")
     wq, wk = heads_q * d_head, heads_k * d_head
     rc = ctx.lib.fml_qk_norm_rope_fwd(ctx.h, q and q.ptr, ld_q or wq, q_out and q_out.ptr, ld_q_out or wq, heads_q, k and k.ptr, ld_k or wk,
                                       k_out and k_out.ptr, ld_k_out or wk, heads_k, rows, d_head, gain_q and gain_q.ptr, gain_k and gain_k.ptr,
@@ -234,7 +237,8 @@ def qk_norm_rope_backward(ctx, q, k, dq_out, dk_out, dq, dk, rows, heads_q, head
                           ld_k=None, ld_dq_out=None, ld_dk_out=None, ld_dq=None, ld_dk=None, accumulate=False, scratch=None):
     """Gradients of `qk_norm_rope_forward` (`fml_qk_norm_rope_bwd`); dgain_q and dgain_k are added to, through `scratch` of
     `qk_norm_rope_scratch(d_head)` floats."""
-    _index_buffer(positions, rows, "qk_norm_rope: positions")
+    if positions is not None:
+        _index_buffer(positions, rows, "qk_norm_rope: positions")
     wq, wk = heads_q * d_head, heads_k * d_head
     if scratch is not None and scratch.size < qk_norm_rope_scratch(d_head):
         raise ValueError(f"qk_norm_rope_backward: the scratch buffer needs {qk_norm_rope_scratch(d_head)} floats")
