@@ -234,6 +234,9 @@ class FmlBindings {
   late final fmlSelftestWaitTimeout = lib.lookupFunction<
       Int32 Function(Pointer<FmlCtx>, Int32),
       int Function(Pointer<FmlCtx>, int)>('fml_selftest_wait_timeout');
+  late final fmlSelftestClusterWait = lib.lookupFunction<
+      Int32 Function(Pointer<FmlCtx>, Int32, Int32),
+      int Function(Pointer<FmlCtx>, int, int)>('fml_selftest_cluster_wait');
   late final fmlSelftestPerDeviceOnce = lib.lookupFunction<
       Int32 Function(Int32, Pointer<Int32>),
       int Function(int, Pointer<Int32>)>('fml_selftest_per_device_once');

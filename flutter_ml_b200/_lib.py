@@ -76,6 +76,7 @@ PROTOTYPES = {
     "fml_sync": [fp],
     "fml_device_status": [fp, C.POINTER(i32)],
     "fml_selftest_wait_timeout": [fp, i32],
+    "fml_selftest_cluster_wait": [fp, i32, i32],
     "fml_selftest_per_device_once": [i32, C.POINTER(i32)],
     "fml_alloc": [fp, i64, C.POINTER(fp)],
     "fml_mem_info": [fp, C.POINTER(i64), C.POINTER(i64), C.POINTER(i64)],

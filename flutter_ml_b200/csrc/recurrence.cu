@@ -46,9 +46,11 @@ struct Params {
   float *df, *dx, *dh0;         // backward
   long long ss_in, ts_in, ss_h, ts_h;
   int n_seq, seq_len, dim, ctiles, accumulate;
-  int cluster;                  // CTAs that share the steps of a sequence
+  int cluster;                  // CTAs that share the steps of a sequence, 16 at most; above bit 8: the self test's limit
   int* status;
 };
+// Self test of the wait for a cluster's pairs: CTA 1 sends none, and the others wait for so many microseconds
+constexpr int TEST_SHIFT = 8, TEST_CTA = 1;
 
 // a = 1 / (1 + e), s = 1 - a = e a with e = exp(-f): neither is a difference, both keep their relative precision (4 u of the
 // exponential, 1.2 |f| u of its argument in base 2, 2 u of the reciprocal, u = 2^-24).  Gates below -80 count as -80: e stays
@@ -88,9 +90,9 @@ __device__ __forceinline__ void send_pair(const float2* here, const uint64_t* ba
                : "memory");
 }
 
-// Waits for a set's bytes, WAIT_LIMIT_NS at most: then the status word gets a code, the CTA waits for nothing more, and the
-// results are whatever they are.
-__device__ __forceinline__ void wait_pairs(uint32_t bar, uint32_t parity, volatile int* gave_up, int* status) {
+// Waits for a set's bytes, `limit_ns` at most: then the status word gets a code and the CTA leaves its loop after the round (its
+// partners, which get nothing from it any more, by the same limit); the results are whatever they are.
+__device__ __forceinline__ void wait_pairs(uint32_t bar, uint32_t parity, volatile int* gave_up, int* status, unsigned long long limit_ns) {
   unsigned long long t0 = 0;
   for (uint32_t spins = 0;; spins++) {
     uint32_t ok;
@@ -105,7 +107,7 @@ __device__ __forceinline__ void wait_pairs(uint32_t bar, uint32_t parity, volati
     if (spins == 0) t0 = fml_tc::globaltimer_ns();
     if ((spins & 0xFF) != 0xFF) continue;
     if (*gave_up) return;
-    if (fml_tc::globaltimer_ns() - t0 > fml_tc::WAIT_LIMIT_NS) {
+    if (fml_tc::globaltimer_ns() - t0 > limit_ns) {
       *gave_up = 1;
       atomicCAS(status, 0, WAIT_CODE);
       return;
@@ -201,10 +203,10 @@ __global__ void __launch_bounds__(32 * WARPS, min_ctas(WARPS, TEAM, BWD)) scan_k
   // CTA's of round r + 1, and those were sent when their owners had read round r's.
   __shared__ __align__(16) float2 ctot[TEAM ? 2 : 1][TEAM ? MAX_CLUSTER : 1][CW];
   __shared__ uint64_t arrived[2];                     // counts the bytes of a set
-  __shared__ int gave_up;
+  __shared__ int gave_up[2];                          // a wait for this set has run out
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int ch = (lane % LANES) * VEC, sub = lane / LANES;
-  const int cs = TEAM ? p.cluster : 1, rank = TEAM ? (int)fml_tc::cluster_ctarank() : 0;
+  const int cs = TEAM ? p.cluster & ((1 << TEST_SHIFT) - 1) : 1, rank = TEAM ? (int)fml_tc::cluster_ctarank() : 0;
   const int unit = blockIdx.x / cs;
   const int seq = unit / p.ctiles, c = (unit - seq * p.ctiles) * CW + ch;
   const bool on = c < p.dim;
@@ -225,7 +227,7 @@ __global__ void __launch_bounds__(32 * WARPS, min_ctas(WARPS, TEAM, BWD)) scan_k
   Raw<VEC, SEG, BWD> raw;
   if (TEAM) {
     if (threadIdx.x == 0) {
-      gave_up = 0;
+      gave_up[0] = gave_up[1] = 0;
       for (int i = 0; i < 2; i++) fml_tc::mbar_init(fml_tc::smem_u32(&arrived[i]), 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -286,11 +288,13 @@ __global__ void __launch_bounds__(32 * WARPS, min_ctas(WARPS, TEAM, BWD)) scan_k
       store_row<VEC>(&wtot[buf][warp][1][ch], B);
     }
     __syncthreads();
+    if (TEAM && *(volatile int*)&gave_up[buf ^ 1]) break;   // in the round before: the same verdict for the whole CTA
     float run[VEC];                                   // the state before the lane's steps; `state`: after the round
     if (TEAM) {
       const uint32_t bar = fml_tc::smem_u32(&arrived[buf]);
       if (threadIdx.x == 0) fml_tc::mbar_expect_tx(bar, (uint32_t)(cs * CW * sizeof(float2)));
-      for (int i = threadIdx.x; i < cs * CW; i += 32 * WARPS) {
+      const unsigned test_us = (unsigned)p.cluster >> TEST_SHIFT;
+      for (int i = test_us && rank == TEST_CTA ? cs * CW : (int)threadIdx.x; i < cs * CW; i += 32 * WARPS) {
         const int r = i / CW, k = i - r * CW;
         float At = 1.f, Bt = 0.f;
 #pragma unroll
@@ -301,7 +305,7 @@ __global__ void __launch_bounds__(32 * WARPS, min_ctas(WARPS, TEAM, BWD)) scan_k
         }
         send_pair(&ctot[buf][rank][k], &arrived[buf], r, make_float2(At, Bt));
       }
-      wait_pairs(bar, phase, &gave_up, p.status);
+      wait_pairs(bar, phase, &gave_up[buf], p.status, test_us ? test_us * 1000ull : fml_tc::WAIT_LIMIT_NS);
       phase ^= buf;                                   // each set is used every other round
       for (int r = 0; r < cs; r++)
 #pragma unroll
@@ -462,10 +466,8 @@ int32_t check(fml_ctx* ctx, const Params& p, int32_t form) {
   FML_REQUIRE(ctx, p.n_seq >= 0 && p.seq_len >= 0 && p.seq_len <= (1 << 30) && p.dim >= 1, "fml_gated_recurrence: bad sizes");
   FML_REQUIRE(ctx, (long long)p.n_seq * ((p.dim + 7) / 8) <= (1ll << 27), "fml_gated_recurrence: too many sequences and channels for one call");
   FML_REQUIRE(ctx, p.ss_in >= 0 && p.ts_in >= 0 && p.ss_h >= 0 && p.ts_h >= 0, "fml_gated_recurrence: strides must not be negative");
-  uintptr_t all = 0;
-  for (const void* q : {(const void*)p.f, (const void*)p.x, (const void*)p.h0, (const void*)p.lens, (const void*)p.out, (const void*)p.last, (const void*)p.h,
-                        (const void*)p.dy, (const void*)p.dh_last, (const void*)p.df, (const void*)p.dx, (const void*)p.dh0})
-    all |= reinterpret_cast<uintptr_t>(q);
+  const auto at = [](const void* q) { return reinterpret_cast<uintptr_t>(q); };
+  const uintptr_t all = at(p.f) | at(p.x) | at(p.h0) | at(p.lens) | at(p.out) | at(p.last) | at(p.h) | at(p.dy) | at(p.dh_last) | at(p.df) | at(p.dx) | at(p.dh0);
   FML_REQUIRE(ctx, (all & 3) == 0, "fml_gated_recurrence: misaligned buffer");
   return FML_OK;
 }
@@ -473,7 +475,7 @@ int32_t check(fml_ctx* ctx, const Params& p, int32_t form) {
 template <int WARPS, int LANES, int VEC, int SEG, bool GATED, bool BWD, bool AHEAD, bool TEAM>
 int32_t launch_scan(fml_ctx* ctx, Params& p, int cluster) {
   p.ctiles = (p.dim + LANES * VEC - 1) / (LANES * VEC);
-  p.cluster = cluster;
+  p.cluster = cluster | (p.cluster & ~((1 << TEST_SHIFT) - 1));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((long long)p.n_seq * p.ctiles * cluster));
   cfg.blockDim = dim3(32 * WARPS);
@@ -668,6 +670,26 @@ int32_t fml_gated_recurrence_bwd(fml_ctx* ctx, int32_t form, int32_t n_seq, int3
   FML_REQUIRE(ctx, (dh_last == dh0 && !accumulate) || !ranges_meet(dh_last, ends, dh0, ends), "fml_gated_recurrence_bwd: dh0 overlaps dh_last");
   FML_REQUIRE(ctx, !ranges_meet(h0, ends, dh0, ends), "fml_gated_recurrence_bwd: dh0 overlaps h0");
   return form == FML_RECURRENCE_GATED ? launch<true, true>(ctx, p) : launch<false, true>(ctx, p);
+}
+
+int32_t fml_selftest_cluster_wait(fml_ctx* ctx, int32_t backward, int32_t limit_us) {
+  FML_REQUIRE(ctx, ctx && limit_us > 0 && limit_us <= 1000000, "fml_selftest_cluster_wait: the limit must be 1 .. 1000000 us");
+  FML_ENTER(ctx);
+  FML_REQUIRE(ctx, !ctx->capturing, "fml_selftest_cluster_wait: not while a graph is being recorded");
+  Params p = {};
+  p.n_seq = 1; p.seq_len = 40000; p.dim = 8; p.status = ctx->d_status;   // three rounds of a cluster
+  p.ss_in = p.ss_h = (long long)p.seq_len * p.dim; p.ts_in = p.ts_h = p.dim;
+  p.cluster = limit_us << TEST_SHIFT;
+  const long long n = p.ss_in;
+  float* b = nullptr;
+  int32_t rc = fml_alloc(ctx, 6 * n, &b);
+  if (rc) return rc;
+  rc = fml_zero(ctx, b, 6 * n);
+  p.f = b; p.x = b + n; p.h = p.dy = b + 2 * n; p.out = b + 3 * n; p.df = b + 4 * n; p.dx = b + 5 * n;
+  if (!rc) rc = backward ? launch<true, true>(ctx, p) : launch<true, false>(ctx, p);
+  if (!rc && (p.cluster & ((1 << TEST_SHIFT) - 1)) < 2) rc = fml_fail(ctx, FML_ERR_INVALID, "fml_selftest_cluster_wait: the device forms no clusters");
+  const int32_t freed = fml_free(ctx, b);
+  return rc ? rc : freed;
 }
 
 }  // extern "C"

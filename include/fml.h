@@ -89,6 +89,9 @@ int32_t fml_device_status(fml_ctx* ctx, int32_t* code);
  * signals; after limit_us microseconds it records code 99 and returns.  fml_device_status then reports
  * FML_ERR_TIMEOUT once and the context stays usable.  Nothing faults, traps or hangs. */
 int32_t fml_selftest_wait_timeout(fml_ctx* ctx, int32_t limit_us);
+/* The same for the gated recurrence's clusters (forward, or backward != 0): one CTA of a cluster keeps its results from the
+ * others, which give up after limit_us microseconds; the code is 130. */
+int32_t fml_selftest_cluster_wait(fml_ctx* ctx, int32_t backward, int32_t limit_us);
 /* Host-only self test (no device needed) of the bookkeeping behind one-time kernel set-up: function attributes such
  * as the shared-memory opt-in belong to one device, so the library keeps one "done" flag per (call site, device).
  * Each call passes through such a guard around a counter for `device` and returns the counter in *runs: it must read

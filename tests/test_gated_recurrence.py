@@ -518,3 +518,29 @@ def test_misaligned_addresses_are_refused(ctx):
                     assert call(args[:i] + [off(v, k)] + args[i + 1:]) != 0, (name, i)
                     assert b"misaligned" in ctx.lib.fml_last_error(ctx.h)
     ctx.sync()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("backward", [0, 1])
+def test_a_cluster_that_waits_in_vain_gives_up(backward):
+    """One CTA of a cluster keeps its pairs (the failure is made by what is not sent, not by a fault): the others give up
+    after the limit, the host reads FML_ERR_TIMEOUT with code 130 once, and the context then runs clusters correctly."""
+    import ctypes
+    import time
+    from flutter_ml_b200 import _lib
+    ctx = _lib.Context()
+    ctx.check(ctx.lib.fml_selftest_cluster_wait(ctx.h, backward, 2000))
+    start, code = time.time(), ctypes.c_int32(0)
+    assert ctx.lib.fml_device_status(ctx.h, ctypes.byref(code)) == -4
+    assert code.value == 130 and b"bounded wait expired" in ctx.lib.fml_last_error(ctx.h)
+    assert time.time() - start < 1.0      # limits of 2 ms, not of every round or of the usual wait
+    assert ctx.device_status() == 0
+    c = Case(ctx, 1, 9001, 8)
+    ref, bound, last, blast = forward64(c.f, c.x, c.h0, c.lens, "gated")
+    h, end = c.forward()
+    close(h.numpy()[c.index(c.sh, 1)], ref, bound, "h")
+    close(end.numpy(), last, blast, "h_last")
+    assert ctx.device_status() == 0
+    for bad in (0, -1, 1000001):
+        assert ctx.lib.fml_selftest_cluster_wait(ctx.h, backward, bad) != 0
+    ctx.close()
