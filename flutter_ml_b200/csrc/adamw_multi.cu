@@ -344,7 +344,15 @@ struct fml_adamw_plan {
   int64_t n_blocks = 0;
   uint32_t n_items = 0;
   int bits = 32;
+  bool recorded = false;   // a graph refers to the table and the counter: they are kept until the context goes
+  bool gone = false;
 };
+
+static fml_adamw_plan* find_plan(fml_ctx* ctx, int32_t id) {
+  if (id < 0 || id >= (int32_t)ctx->adamw_plans.size()) return nullptr;
+  fml_adamw_plan* p = ctx->adamw_plans[id];
+  return p && !p->gone ? p : nullptr;
+}
 
 static void free_plan(fml_adamw_plan* p) {
   if (p->items) cudaFree(p->items);
@@ -434,7 +442,8 @@ int32_t fml_adamw_plan_step(fml_ctx* ctx, int32_t plan_id, int32_t lane, double 
                             double weight_decay, int32_t t, double grad_scale, int32_t zero_grad, int64_t seed) {
   FML_REQUIRE(ctx, ctx, "fml_adamw_plan_step: no context");
   FML_ENTER(ctx);
-  FML_REQUIRE(ctx, plan_id >= 0 && plan_id < (int32_t)ctx->adamw_plans.size() && ctx->adamw_plans[plan_id], "fml_adamw_plan_step: unknown plan");
+  fml_adamw_plan* p = find_plan(ctx, plan_id);
+  FML_REQUIRE(ctx, p, "fml_adamw_plan_step: unknown plan");
   FML_REQUIRE(ctx, beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, "fml_adamw_plan_step: betas must be in [0, 1)");
   FML_REQUIRE(ctx, eps >= 1e-37 && isfinite(eps) && isfinite(lr) && isfinite(weight_decay) && isfinite(grad_scale),
               "fml_adamw_plan_step: hyper-parameters must be finite, eps at least 1e-37");
@@ -442,7 +451,9 @@ int32_t fml_adamw_plan_step(fml_ctx* ctx, int32_t plan_id, int32_t lane, double 
   cudaStream_t s;
   const int32_t rc = fml_any_stream(ctx, lane, &s);
   if (rc) return rc;
-  const fml_adamw_plan* p = ctx->adamw_plans[plan_id];
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;   // also of a stream that the caller records
+  FML_CUDA(ctx, cudaStreamIsCapturing(s, &capture));
+  p->recorded |= capture != cudaStreamCaptureStatusNone;
   const HyperIn in = {lr, beta1, beta2, eps, weight_decay, grad_scale, seed};
   const DeviceStep* dev = nullptr;
   if (t == 0) {
@@ -462,10 +473,11 @@ int32_t fml_adamw_plan_step(fml_ctx* ctx, int32_t plan_id, int32_t lane, double 
 // The plan's own counter, once every step enqueued so far has run, on whatever stream
 static int32_t counter(fml_ctx* ctx, int32_t plan_id, int* t, bool set) {
   FML_ENTER(ctx);
-  FML_REQUIRE(ctx, plan_id >= 0 && plan_id < (int32_t)ctx->adamw_plans.size() && ctx->adamw_plans[plan_id], "fml_adamw_plan_count: unknown plan");
+  fml_adamw_plan* p = find_plan(ctx, plan_id);
+  FML_REQUIRE(ctx, p, "fml_adamw_plan_count: unknown plan");
   FML_REQUIRE(ctx, !ctx->capturing, "fml_adamw_plan_count: not while a graph is being recorded");
   FML_CUDA(ctx, cudaDeviceSynchronize());
-  int* at = &ctx->adamw_plans[plan_id]->step->t;
+  int* at = &p->step->t;
   FML_CUDA(ctx, set ? cudaMemcpy(at, t, sizeof(int), cudaMemcpyHostToDevice) : cudaMemcpy(t, at, sizeof(int), cudaMemcpyDeviceToHost));
   if (set) FML_CUDA(ctx, cudaDeviceSynchronize());
   return FML_OK;
@@ -484,10 +496,15 @@ int32_t fml_adamw_plan_set_count(fml_ctx* ctx, int32_t plan_id, int32_t t) {
 int32_t fml_adamw_plan_destroy(fml_ctx* ctx, int32_t plan_id) {
   FML_REQUIRE(ctx, ctx, "fml_adamw_plan_destroy: no context");
   FML_ENTER(ctx);
-  FML_REQUIRE(ctx, plan_id >= 0 && plan_id < (int32_t)ctx->adamw_plans.size() && ctx->adamw_plans[plan_id], "fml_adamw_plan_destroy: unknown plan");
+  fml_adamw_plan* p = find_plan(ctx, plan_id);
+  FML_REQUIRE(ctx, p, "fml_adamw_plan_destroy: unknown plan");
   FML_REQUIRE(ctx, !ctx->capturing, "fml_adamw_plan_destroy: not while a graph is being recorded");
   FML_CUDA(ctx, cudaDeviceSynchronize());   // steps may still run on the main stream or on any lane
-  free_plan(ctx->adamw_plans[plan_id]);
+  if (p->recorded) {
+    p->gone = true;
+    return FML_OK;
+  }
+  free_plan(p);
   ctx->adamw_plans[plan_id] = nullptr;
   return FML_OK;
 }

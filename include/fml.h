@@ -355,8 +355,9 @@ int32_t fml_optimizer_step(fml_ctx* ctx, int32_t kind, float* w, const float* g,
  *                for minus infinity), then one float32 scale, a power of two, for each block; an element is code * scale,
  *                and the second buffer holds sqrt(v).
  * Steps of one plan follow each other (they update the same buffers); different plans may run at once on different lanes.
- * A plan belongs to its context, which frees those that are left at fml_shutdown; it must outlive the graphs that were
- * recorded with it.  Make and destroy plans outside recordings (both wait for the device). */
+ * A plan belongs to its context, which frees those that are left at fml_shutdown.  The table of a plan that was recorded
+ * into a graph is kept until then, also when the plan is destroyed: the graph's replays go on updating the same buffers,
+ * which stay the caller's to keep.  Make and destroy plans outside recordings (both wait for the device). */
 int32_t fml_adamw_state_floats(int32_t n, const int64_t* sizes, int32_t state_bits, int64_t* floats);
 int32_t fml_adamw_plan_create(fml_ctx* ctx, int32_t n, float* const* w, float* const* g, const int64_t* sizes, float* m,
                               float* v, int32_t state_bits, int32_t* plan_id);

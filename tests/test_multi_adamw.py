@@ -557,3 +557,53 @@ def test_training_goes_on_from_a_checkpoint(ctx, tmp_path, bits, device):
     oa._plan.close()
     with pytest.raises(Exception, match="unknown plan"):
         oa._plan.count
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_recording_outlives_its_plan(ctx, bits):
+    """The plan is destroyed, others take the place of what it could have freed, and the recording is replayed: it updates
+    what the plan updated, as steps with t = 1, 2, 3 do."""
+    a, b = Setup(ctx, [700, 3000], bits, seed=6), Setup(ctx, [700, 3000], bits, seed=6)
+    ctx.sync()
+    ctx.graph_begin()
+    a.step(0, seed=11)
+    gid = ctx.graph_end()
+    a.plan.close()
+    with pytest.raises(Exception, match="unknown plan"):
+        a.plan.count
+    others = [Setup(ctx, [700, 3000], bits, seed=i) for i in range(4)]
+    for t in (1, 2, 3):
+        ctx.graph_launch(gid)
+        b.step(t, seed=11)
+        for o in others:
+            o.step(t)
+    ctx.sync()
+    assert np.array_equal(a.m.numpy().view(np.int32), b.m.numpy().view(np.int32))
+    assert np.array_equal(a.v.numpy().view(np.int32), b.v.numpy().view(np.int32))
+    ctx.check(ctx.lib.fml_graph_destroy(ctx.h, gid))
+
+
+@pytest.mark.gpu
+def test_a_recorded_step_outlives_a_moved_gradient(ctx):
+    """MultiTensorAdamW makes its plan anew where a gradient has moved; a recording of the step before goes on with the old
+    addresses."""
+    from flutter_ml_b200 import optimizers as O
+    from flutter_ml_b200.tensor import Tensor
+    p = Tensor(np.ones(3000, f32), ctx)
+    p.grad = first = ctx.upload(np.full(3000, 0.5, f32))
+    opt = O.MultiTensorAdamW([p], 0.01)
+    ctx.sync()
+    ctx.graph_begin()
+    opt.step()
+    gid = ctx.graph_end()
+    old = opt._plan
+    p.grad = ctx.upload(np.full(3000, 0.5, f32))
+    opt.step()
+    assert opt._plan is not old and old.id == -1
+    once = p.numpy()
+    ctx.zero(p.grad)                    # the recording reads the gradient that it was made with
+    ctx.graph_launch(gid)
+    ctx.sync()
+    assert (p.numpy() < once).all() and first.size == 3000
+    ctx.check(ctx.lib.fml_graph_destroy(ctx.h, gid))
