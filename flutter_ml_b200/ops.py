@@ -282,8 +282,9 @@ class AdamWPlan:
             raise _lib.FmlError(lib.fml_last_error(None).decode())
         return out.value
 
-    def step(self, lr, beta1, beta2, epsilon, weightDecay, t, grad_scale=1.0, zero_grad=False, seed=-1, lane=-1):
-        """One update; t = 0 counts on the device (for recorded steps), seed >= 0 rounds 8-bit states at random."""
+    def step(self, lr, beta1, beta2, epsilon, weightDecay, t, grad_scale=1.0, zero_grad=False, seed=0, lane=-1):
+        """One update; t = 0 counts on the device (for recorded steps).  8-bit states are rounded at random by `seed`, or to
+        the nearest code where it is negative, which with a beta2 near 1 is not AdamW (see `fml_adamw_plan_step`)."""
         self.ctx.check(self.ctx.lib.fml_adamw_plan_step(self.ctx.h, self.id, lane, lr, beta1, beta2, epsilon, weightDecay, t, grad_scale,
                                                         1 if zero_grad else 0, seed))
         self.ctx.launches += 1 if t else 2

@@ -217,7 +217,8 @@ class MultiTensorAdamW(Optimizer):
     moments in 32 bits or in 8 (a quarter of the state memory; `fml_adamw_plan_create` describes the format).
 
     stateBits=8 rounds the moments at random by `seed` (the same seed repeats a run exactly) unless `seed` is None, which
-    rounds to the nearest code.  Gradients that do not exist yet are created, zeroed, here.  `step()` looks at the tensors'
+    rounds to the nearest code: not for training with a beta2 near 1, where second moments rounded that way stand still
+    and steps become two to three times as long.  Gradients that do not exist yet are created, zeroed, here.  `step()` looks at the tensors'
     and gradients' addresses and makes its plan anew where one has changed.  deviceCounter=True keeps the step count on the
     device, so that a recorded step (`graph_begin`) advances it at every replay; `checkpoint.save_training_state` and
     `load_training_state` read and set it there."""

@@ -363,9 +363,12 @@ int32_t fml_adamw_plan_create(fml_ctx* ctx, int32_t n, float* const* w, float* c
                               float* v, int32_t state_bits, int32_t* plan_id);
 /* One step on copy lane `lane` (-1: the main stream).  t >= 1 is the step count after the increment, as in fml_adam_step;
  * t = 0 counts the plan's steps on the device, so that every replay of a recorded step advances the count.  grad_scale
- * multiplies g first; zero_grad != 0 clears g in the same pass.  seed concerns 8-bit states only: negative rounds to the
- * nearest code, any other value rounds up or down at random with the probabilities that keep the mean, from a generator
- * over (seed, t, block, element) - the same call gives the same bits.  eps must be 1e-37 or more, betas in [0, 1). */
+ * multiplies g first; zero_grad != 0 clears g in the same pass.  seed concerns 8-bit states only: a value of 0 or more rounds
+ * up or down at random with the probabilities that keep the mean, from a generator over (seed, t, block, element) - the
+ * same call gives the same bits.  A negative one rounds to the nearest code; that is for single steps and comparisons, not
+ * for training with a beta2 near 1: a step that changes a root by less than half a code (1/16) leaves it where it is, so
+ * with 0.999 it settles at less than half of AdamW's (steps of 2.5 times AdamW's).  eps must be 1e-37 or more, betas in
+ * [0, 1). */
 int32_t fml_adamw_plan_step(fml_ctx* ctx, int32_t plan_id, int32_t lane, double lr, double beta1, double beta2, double eps,
                             double weight_decay, int32_t t, double grad_scale, int32_t zero_grad, int64_t seed);
 /* The number of steps with t = 0 so far (a new plan: 0), for a checkpoint, and setting it, to go on from one.  Both wait
