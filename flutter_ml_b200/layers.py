@@ -234,6 +234,8 @@ class GatedRecurrentLayer(Layer):
         super().build(x)
 
     def forward(self, x: Tensor, lens=None, h0: Optional[Tensor] = None) -> Tensor:
+        if not self._built:
+            self.build(x)
         S = self.seq_len or x.shape[0]
         z = T.denseMatrix(x, self.weights, self.biases, None, self.precision)
         return T.gatedRecurrence(z, x.shape[0] // S, S, "gated", h0, lens, "all" if self.returnSequences else "last")

@@ -544,3 +544,16 @@ def test_a_cluster_that_waits_in_vain_gives_up(backward):
     for bad in (0, -1, 1000001):
         assert ctx.lib.fml_selftest_cluster_wait(ctx.h, backward, bad) != 0
     ctx.close()
+
+
+@pytest.mark.gpu
+def test_ragged_sequences_may_come_first(ctx):
+    """`forward` with lengths is the only way to hand over ragged sequences, so it may be the layer's first call."""
+    from flutter_ml_b200 import layers, synth
+    from flutter_ml_b200 import tensor as T
+    x, lens = T.Tensor(synth.normal(1, 0, (20, 6)), ctx), ctx.upload(np.array([10, 4], np.int32))
+    first, built = (layers.GatedRecurrentLayer(8, seq_len=10, seed=2) for _ in range(2))
+    built.build(x)
+    y = first.forward(x, lens=lens).numpy()
+    assert np.array_equal(y, built.forward(x, lens=lens).numpy()) and not y[14:].any() and y[:14].any()
+    assert [p.shape for p in first.parameters] == [(6, 16), (16,)]
