@@ -487,3 +487,73 @@ def test_misaligned_addresses_are_refused(ctx):
                     assert call(args[:i] + [ctypes.c_void_p(v.value + k)] + args[i + 1:]) != 0, (name, i)
                     assert b"misaligned" in ctx.lib.fml_last_error(ctx.h)
     ctx.sync()
+
+
+# ---- gain gradients against a bound from the additions that a term really passes through
+GAINS = [dict(rows=20000, hq=2, hk=1, d=64, rot=64, positions=512),                 # every place taken, two rounds of angles a CTA
+         dict(rows=4999, hq=12, hk=3, d=80, rot=32, interleaved=True, pad=7),
+         dict(rows=9001, hq=3, hk=3, d=128, rot=128, positions=1000),
+         dict(rows=6000, hq=5, hk=2, d=24, rot=8),
+         dict(rows=5000, hq=2, hk=2, d=256, rot=0, positions=0),
+         dict(rows=3001, hq=1, hk=1, d=10, rot=6),                                    # pairs
+         dict(rows=7000, hq=3, hk=2, d=100, rot=100, positions=64)]
+
+
+def shares(case, sms):
+    """(grid, first row of each CTA's share and the end, rows at once) of a backward launch."""
+    rows, heads = case["rows"], max(case["hq"], case["hk"])
+    grid = min(rows, 3 * sms, 592)
+    first = [rows // grid * b + min(b, rows % grid) for b in range(grid + 1)]
+    return grid, first, min(32, 8192 // max(case["rot"], 1), -(-rows // grid), max(1, 2 ** 31 // heads ** 2))
+
+
+def additions(case, t, sms):
+    """Additions on a term's way into the gain gradient of queries (t = 0) or keys: its lane's items, the heads beside it in
+    the warp, the warps, the partial sums of the second kernel, its shuffles, the old value."""
+    grid, first, at_once = shares(case, sms)
+    d, heads = case["d"], (case["hq"], case["hk"])
+    share = max(b - a for a, b in zip(first, first[1:]))
+    groups = [min(at_once, share - r) for r in range(0, share, at_once)]
+    if d % 8 or case["rot"] % 8:
+        return sum(-(-n * sum(heads) // 8) for n in groups) + 8 + 19 + 5 + 1
+    beside = 32 // (4 if d <= 32 else 8 if d <= 64 else 16 if d <= 128 else 32)
+    return sum(-(-n * heads[t] // (8 * beside)) for n in groups) + int(np.log2(beside)) + 8 + 19 + 5 + 1
+
+
+def gain_gradient(c, t, sms, case):
+    """The reference, and its bound: 30 u of each term (16 more at far positions), and one rounding an addition."""
+    r = c.ref(t, True)
+    far = 16 if np.abs(c.pos).max() > 1 << 20 else 0
+    terms = r[5] / ((c.rows * c.h[t] + 50 + far) * U)          # the sum of D |xh|
+    return r[4], (30 + far + additions(case, t, sms)) * U * terms
+
+
+@pytest.mark.parametrize("case", GAINS, ids=lambda c: "-".join(str(v) for v in c.values()))
+def test_the_gain_bound_sees_a_lost_share(case):
+    """Without the rows of one CTA, the first, the last or one between, or without the second round of a CTA's rows, the gain
+    gradients are off by more than the bound in most columns."""
+    from types import SimpleNamespace
+    c = Case(SimpleNamespace(upload=lambda a, **kw: a), **case)
+    grid, first, at_once = shares(case, 148)
+    lost = [(first[b], first[b + 1]) for b in (0, grid // 2, grid - 1)]
+    if first[1] > at_once:
+        lost.append((first[1] - (first[1] - at_once), first[1]))
+    for t in range(2):
+        want, bound = gain_gradient(c, t, 148, case)
+        for a, b in lost:
+            kept = np.r_[0:a, b:c.rows]
+            g = c.gains[t].astype(np.float64)
+            x, dy = c.side(t)[kept], c.dy[t].reshape(c.rows, c.h[t], c.d).astype(np.float64)[kept]
+            less = reference(x, g, c.pos[kept], c.rot, c.inter, c.base, c.eps, dy)[4]
+            assert np.mean(np.abs(less - want) > 3 * bound) > 0.8, (t, a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", GAINS, ids=lambda c: "-".join(str(v) for v in c.values()))
+def test_gain_gradients_of_whole_grids(ctx, case):
+    c = Case(ctx, **case)
+    dg = [ctx.zeros(c.d), ctx.zeros(c.d)]
+    c.backward(ctx.zeros(c.host.size), dg)
+    for t in range(2):
+        want, bound = gain_gradient(c, t, ctx.sm_count(), case)
+        close(dg[t].numpy(), want, bound, "gain gradient")
