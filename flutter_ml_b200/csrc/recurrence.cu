@@ -90,9 +90,9 @@ __device__ __forceinline__ void send_pair(const float2* here, const uint64_t* ba
                : "memory");
 }
 
-// Waits for a set's bytes, `limit_ns` at most: then the status word gets a code and the CTA leaves its loop after the round (its
-// partners, which get nothing from it any more, by the same limit); the results are whatever they are.
-__device__ __forceinline__ void wait_pairs(uint32_t bar, uint32_t parity, volatile int* gave_up, int* status, unsigned long long limit_ns) {
+// Waits for a set's bytes, `limit_ns` at most: false when they did not come, or not for another thread of the CTA.  The status
+// word then has a code, and the results are whatever they are.
+__device__ __forceinline__ bool wait_pairs(uint32_t bar, uint32_t parity, volatile int* gave_up, int* status, unsigned long long limit_ns) {
   unsigned long long t0 = 0;
   for (uint32_t spins = 0;; spins++) {
     uint32_t ok;
@@ -103,14 +103,14 @@ __device__ __forceinline__ void wait_pairs(uint32_t bar, uint32_t parity, volati
         : "=r"(ok)
         : "r"(bar), "r"(parity)
         : "memory");
-    if (ok) return;
+    if (ok) return true;
     if (spins == 0) t0 = fml_tc::globaltimer_ns();
     if ((spins & 0xFF) != 0xFF) continue;
-    if (*gave_up) return;
+    if (*gave_up) return false;
     if (fml_tc::globaltimer_ns() - t0 > limit_ns) {
       *gave_up = 1;
       atomicCAS(status, 0, WAIT_CODE);
-      return;
+      return false;
     }
   }
 }
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(32 * WARPS, min_ctas(WARPS, TEAM, BWD)) scan_k
   // CTA's of round r + 1, and those were sent when their owners had read round r's.
   __shared__ __align__(16) float2 ctot[TEAM ? 2 : 1][TEAM ? MAX_CLUSTER : 1][CW];
   __shared__ uint64_t arrived[2];                     // counts the bytes of a set
-  __shared__ int gave_up[2];                          // a wait for this set has run out
+  __shared__ int gave_up;                             // a thread's wait has run out
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int ch = (lane % LANES) * VEC, sub = lane / LANES;
   const int cs = TEAM ? p.cluster & ((1 << TEST_SHIFT) - 1) : 1, rank = TEAM ? (int)fml_tc::cluster_ctarank() : 0;
@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(32 * WARPS, min_ctas(WARPS, TEAM, BWD)) scan_k
   Raw<VEC, SEG, BWD> raw;
   if (TEAM) {
     if (threadIdx.x == 0) {
-      gave_up[0] = gave_up[1] = 0;
+      gave_up = 0;
       for (int i = 0; i < 2; i++) fml_tc::mbar_init(fml_tc::smem_u32(&arrived[i]), 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -236,6 +236,7 @@ __global__ void __launch_bounds__(32 * WARPS, min_ctas(WARPS, TEAM, BWD)) scan_k
   int p0 = ((rank * WARPS + warp) * SUBS + sub) * SEG;   // first step of the segment, counted in scan direction
   if (AHEAD) load_segment<VEC, SEG, GATED, BWD>(p, raw, f, x, h, dy, first, p0, len, on);
   uint32_t phase = 0;
+  bool arriving = true;                               // a thread that has waited in vain waits, and arms a barrier, no more
   for (int base = 0, buf = 0; base < len; base += TILE * cs, p0 += TILE * cs, buf ^= 1) {
     if (!AHEAD) load_segment<VEC, SEG, GATED, BWD>(p, raw, f, x, h, dy, first, p0, len, on);
     // forward: decay and input; backward: decay, incoming gradient, and what G is multiplied by for dx and df
@@ -288,13 +289,12 @@ __global__ void __launch_bounds__(32 * WARPS, min_ctas(WARPS, TEAM, BWD)) scan_k
       store_row<VEC>(&wtot[buf][warp][1][ch], B);
     }
     __syncthreads();
-    if (TEAM && *(volatile int*)&gave_up[buf ^ 1]) break;   // in the round before: the same verdict for the whole CTA
     float run[VEC];                                   // the state before the lane's steps; `state`: after the round
     if (TEAM) {
       const uint32_t bar = fml_tc::smem_u32(&arrived[buf]);
-      if (threadIdx.x == 0) fml_tc::mbar_expect_tx(bar, (uint32_t)(cs * CW * sizeof(float2)));
+      if (threadIdx.x == 0 && arriving) fml_tc::mbar_expect_tx(bar, (uint32_t)(cs * CW * sizeof(float2)));
       const unsigned test_us = (unsigned)p.cluster >> TEST_SHIFT;
-      for (int i = test_us && rank == TEST_CTA ? cs * CW : (int)threadIdx.x; i < cs * CW; i += 32 * WARPS) {
+      for (int i = !arriving || (test_us && rank == TEST_CTA) ? cs * CW : (int)threadIdx.x; i < cs * CW; i += 32 * WARPS) {
         const int r = i / CW, k = i - r * CW;
         float At = 1.f, Bt = 0.f;
 #pragma unroll
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(32 * WARPS, min_ctas(WARPS, TEAM, BWD)) scan_k
         }
         send_pair(&ctot[buf][rank][k], &arrived[buf], r, make_float2(At, Bt));
       }
-      wait_pairs(bar, phase, &gave_up[buf], p.status, test_us ? test_us * 1000ull : fml_tc::WAIT_LIMIT_NS);
+      if (arriving) arriving = wait_pairs(bar, phase, &gave_up, p.status, test_us ? test_us * 1000ull : fml_tc::WAIT_LIMIT_NS);
       phase ^= buf;                                   // each set is used every other round
       for (int r = 0; r < cs; r++)
 #pragma unroll
