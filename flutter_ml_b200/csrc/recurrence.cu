@@ -16,13 +16,14 @@
 // with "state <- A state + B"; the pairs are joined across the lanes of the same channels by shuffles, across the warps of the
 // CTA through shared memory, across the CTAs of a cluster (which split the steps when there are too few channels to fill the
 // GPU) by asynchronous stores into one another's shared memory; then every lane runs its own steps again from the state it
-// now knows, in registers, and writes.  The data crosses the memory bus once.  The order of all joins depends on the sizes
-// alone: results repeat bit for bit.  Single steps (token by token use) and other very short sequences take one thread a channel.
+// now knows, in registers, and writes.  The data crosses the memory bus once.  The order of all joins depends on the sizes, the
+// addresses and strides (which decide how wide the loads are) and the device (how many clusters it holds), never on timing: a
+// call repeats bit for bit.  Single steps (token by token use) and other very short sequences take one thread a channel.
 //
 // Measured (us; bytes at the copy's rate in brackets): 128 sequences of 128 x 512 forward 18 (15); 32 ragged ones of 512 x 1024
-// 21 forward (14), 37 backward (29); 8 of 2048 x 1024 36 (31) and 69 (61); one of 16384 x 1024, in clusters of four, 44 (31) and
-// 78 (61); one of 65521 x 250, in clusters of thirteen, LINEAR, 58 (30) and 96 (50); one of 52433 x 192, in clusters of sixteen,
-// 42 (18) and 73 (37).  The first are bound by memory, with about 5 us for the first loads and last stores; the clusters by the
+// 21 forward (14), 37 backward (29); 8 of 2048 x 1024 35 (31) and 69 (61); one of 16384 x 1024, in clusters of four, 44 (31) and
+// 80 (61); one of 65521 x 250, in clusters of thirteen, LINEAR, 57 (30) and 95 (50); one of 52433 x 192, in clusters of sixteen,
+// 43 (18) and 75 (37).  The first are bound by memory, with about 5 us for the first loads and last stores; the clusters by the
 // chain of a round, which 16 warps an SM do not hide.
 #include <math.h>
 
@@ -136,7 +137,8 @@ __device__ __forceinline__ void store_row(float* dst, const float* src) {
 }
 
 // CTAs an SM that a scan is compiled for.  Forward 128 registers a thread (128 sequences of 128 x 512: 18.5 us; left alone the
-// compiler takes 200 and it is 23).  Backward the next round's four rows need them: 35 us with any number, 47 with 128.
+// compiler takes 200 and it is 23).  Backward the next round's four rows need them: 35 us with any number, 47 with 128.  At 128
+// registers sixteen of the 120 instances spill 4 to 8 bytes, five forward ones of four channels a lane 12 to 48.
 constexpr int min_ctas(int warps, bool team, bool bwd) { return team ? 2 : bwd ? 1 : 16 / warps; }
 
 // What a lane has read of its segment, SEG steps of VEC channels, in scan direction.
@@ -534,7 +536,7 @@ int32_t clusters_at_once(fml_ctx* ctx, int size, long long* out) {
 // Few channels: eight warps, rows of LANES, long segments forward, and a cluster along the steps: two CTAs an SM, or where eight
 // CTAs a cluster do not give one an SM, up to sixteen and one and a half; no more of them than the same number of rounds needs,
 // and only as many as let all clusters run at once.
-// One sequence of 16384 x 1024: 44 and 78 us with four, of 52433 x 192: 42 and 73 with sixteen (56 and 105 with eight), of
+// One sequence of 16384 x 1024: 44 and 80 us with four, of 52433 x 192: 43 and 75 with sixteen (56 and 105 with eight), of
 // 18285 x 256: 21 and 37 with twelve (27 and 44).  14 of 2899 x 112, 98 units of which 93 clusters of three run at once: 19 and
 // 33 with two, 23 and 37 with three.
 template <int LANES, int VEC, bool GATED, bool BWD>
@@ -563,7 +565,7 @@ int32_t launch_lanes(fml_ctx* ctx, Params& p) {
   // Channels enough: each CTA goes over all steps of its channels, the next round's rows in registers meanwhile.  Rows as wide as
   // leave three to four CTAs of four warps an SM, at least 32 channels of them, else eight warps.  Measured (us, forward and
   // backward): 128 sequences of 128 x 512, 32 lanes of four: 18 and 35.  32 of 512 x 1024: 34 and 65 with 16 lanes, 35 and 68
-  // with 8; ragged 25 and 37, 21 and 37.  8 of 2048 x 1024, eight warps of 8 lanes: 36 and 69, four warps 49 and 68.  Two
+  // with 8; ragged 25 and 37, 21 and 37 (the one ragged size that was compared).  8 of 2048 x 1024, eight warps of 8 lanes: 36 and 69, four warps 49 and 68.  Two
   // channels a lane, 8 of 2048 x 1022: eight warps of 16 lanes 37 and 74, of 8 40 and 84.  One, 32 of 512 x 1001: 32 lanes 39
   // and 84, 8 46 and 108; 100 of 300 x 77: 16 lanes 10 and 20, 8 13 and 29.
 #define FML_SCAN(warps, lanes) return launch_scan<warps, lanes, VEC, SEG, GATED, BWD, true, false>(ctx, p, 1)
