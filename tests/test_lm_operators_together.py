@@ -132,3 +132,44 @@ def test_token_by_token(ctx):
         out = o @ m.att.Wo.numpy().astype(np.float64)
         assert np.linalg.norm(h.numpy() - h_all[:, t]) <= 1e-5 * np.linalg.norm(h_all[:, t])
         assert np.linalg.norm(out - att_all[:, t]) <= 1e-5 * np.linalg.norm(att_all[:, t])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_recorded_training_step(ctx, bits):
+    """Loss, backward pass and optimizer step recorded once and replayed three times, against the same three steps launched one
+    by one from the same place: the same parameters, gradients and moments, bit for bit."""
+    import gc
+    from flutter_ml_b200 import optimizers, tensor as T
+    x0, y0 = data()
+
+    def start():
+        x, target = T.Tensor(x0, ctx), T.Tensor(y0, ctx)
+        m = Model(ctx, x)
+        opt = optimizers.MultiTensorAdamW(m.parameters, 0.01, stateBits=bits, seed=5, deviceCounter=True)
+
+        def step():
+            m.loss(x, target).backward()
+            x.grad = m.att.lastAttentionWeights = None      # nothing of one step is freed in the next
+            opt.step(zero_grad=True)
+        step()
+        gc.collect()
+        return m, opt, step
+    a, oa, step_a = start()
+    b, ob, step_b = start()
+    for _ in range(3):
+        step_a()
+    ctx.sync()
+    gc.collect()                        # what was allocated outside the recording is not freed inside it
+    ctx.graph_begin()
+    step_b()
+    gc.collect()                        # what the recording allocated is freed inside it
+    gid = ctx.graph_end()
+    for _ in range(3):
+        ctx.graph_launch(gid)
+    ctx.sync()
+    assert oa._t == ob._t == 4
+    for p, q in zip(a.parameters, b.parameters):
+        assert np.array_equal(p.numpy(), q.numpy()) and np.array_equal(p.grad.numpy(), q.grad.numpy())
+    for p, q in ((oa._m, ob._m), (oa._v, ob._v)):
+        assert np.array_equal(p.numpy().view(np.int32), q.numpy().view(np.int32))
+    ctx.check(ctx.lib.fml_graph_destroy(ctx.h, gid))
