@@ -27,8 +27,9 @@
 // reproduces the codes bit for bit; the root is the rounded one.
 //
 // Measured on 141 M parameters: 32 bits 566 us, 7.0 TB/s; 8 bits 382 us (5.9 TB/s) at the full clock, 403 to 418 where the
-// power cap lowers it: about 64 instructions an element, 0.8 of the issue slots, 4 to 20 bytes spilled at 48 registers.  The first form, codes taken apart by
-// shifts and selections, took 549.  Persistent CTAs with the next block in registers: 460 (two CTAs an SM).
+// power cap lowers it: about 64 instructions an element, 0.8 of the issue slots, 4 to 20 bytes spilled at 48 registers.  The
+// first form, codes taken apart by shifts and selections, took 549.  Persistent CTAs with the next block in registers: 460
+// (two CTAs an SM).
 #include <math.h>
 
 #include <algorithm>

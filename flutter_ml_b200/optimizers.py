@@ -218,10 +218,10 @@ class MultiTensorAdamW(Optimizer):
 
     stateBits=8 rounds the moments at random by `seed` (the same seed repeats a run exactly) unless `seed` is None, which
     rounds to the nearest code: not for training with a beta2 near 1, where second moments rounded that way stand still
-    and steps become two to three times as long.  Gradients that do not exist yet are created, zeroed, here.  `step()` looks at the tensors'
-    and gradients' addresses and makes its plan anew where one has changed.  deviceCounter=True keeps the step count on the
-    device, so that a recorded step (`graph_begin`) advances it at every replay; `checkpoint.save_training_state` and
-    `load_training_state` read and set it there."""
+    and steps become two to three times as long.  Gradients that do not exist yet are created, zeroed, here.  `step()`
+    looks at the tensors' and gradients' addresses and makes its plan anew where one has changed.  deviceCounter=True keeps
+    the step count on the device, so that a recorded step (`graph_begin`) advances it at every replay;
+    `checkpoint.save_training_state` and `load_training_state` read and set it there."""
 
     def __init__(self, parameters, learningRate, beta1=0.9, beta2=0.999, epsilon=1e-8, weightDecay=0.01, stateBits=32,
                  seed: Optional[int] = 0, deviceCounter: bool = False):

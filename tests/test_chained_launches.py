@@ -77,3 +77,51 @@ def test_a_chain_is_its_calls_one_at_a_time(ctx, bits):
     for _ in range(3):
         for a, b in zip(run(False), want):
             assert np.array_equal(a, b)
+
+
+@pytest.mark.gpu
+def test_recorded_by_the_owner_of_the_stream():
+    """The context works on a stream that torch owns and records: recurrence (in clusters, their first use), norm and optimizer
+    step replayed three times against three eager rounds, also when the plan has been destroyed in between."""
+    import torch
+    from flutter_ml_b200 import _lib, ops
+    S, W, d = 6000, 128, 64
+    rng = np.random.default_rng(3)
+    z0, dy0 = rng.standard_normal((S, 2 * W)).astype(f32), rng.standard_normal((S, W)).astype(f32)
+
+    def run(record):
+        stream = torch.cuda.Stream()
+        ctx = _lib.Context()
+        ctx.check(ctx.lib.fml_set_stream(ctx.h, stream.cuda_stream))
+        z, dy, h, y, dz = ctx.upload(z0), ctx.upload(dy0), ctx.zeros(S, W), ctx.zeros(S, W), ctx.zeros(S, 2 * W)
+        n = ops.AdamWPlan.state_floats([z.size], 8)
+        m, v = ctx.zeros(n), ctx.zeros(n)
+        plan = ops.AdamWPlan(ctx, [z], [dz], m, v, 8)
+
+        def step():
+            st = dict(strides_in=(S * 2 * W, 2 * W))
+            ops.gated_recurrence_forward(ctx, z, z.view(W, ()), h, 1, S, W, **st)
+            ops.qk_norm_rope_forward(ctx, h, h.view(d, ()), y, y.view(d, ()), S, 1, 1, d, ld_q=W, ld_k=W, ld_q_out=W, ld_k_out=W)
+            ops.gated_recurrence_backward(ctx, z, z.view(W, ()), h, dy, dz, dz.view(W, ()), 1, S, W, **st)
+            plan.step(0.01, 0.9, 0.999, 1e-8, 0.0, 0, seed=2)
+        ctx.sync()
+        if record:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                step()
+            plan.close()
+            with torch.cuda.stream(stream):
+                for _ in range(3):
+                    graph.replay()
+        else:
+            for _ in range(3):
+                step()
+        ctx.sync()
+        out = [b.numpy().view(np.int32) for b in (z, h, y, dz, m, v)]
+        assert ctx.device_status() == 0
+        if record:
+            graph.reset()
+        ctx.close()
+        return out
+    for a, b in zip(run(True), run(False)):
+        assert np.array_equal(a, b)
